@@ -835,6 +835,21 @@ static EncodeTiledFn tensor_map_encoder()
     return fn;
 }
 
+bool encode_map_tiled(void* out128, int elemBytes, const void* base, long long inner, long long outer, long long strideBytes, int boxInner, int boxOuter,
+                      bool swizzle128)
+{
+    EncodeTiledFn enc = tensor_map_encoder();
+    if (!enc)
+        return false;
+    const cuuint64_t dims[2] = {(cuuint64_t) inner, (cuuint64_t) outer};
+    const cuuint64_t strides[1] = {(cuuint64_t) strideBytes};
+    const cuuint32_t box[2] = {(cuuint32_t) boxInner, (cuuint32_t) boxOuter};
+    const cuuint32_t estr[2] = {1, 1};
+    return enc(static_cast<CUtensorMap*>(out128), elemBytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims,
+               strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // map of a column-major M x N fp32 matrix with a box of boxRows rows x boxCols columns; false if it cannot be encoded
 bool encode_map_2d(void* out128, const float* base, long long M, long long N, int boxRows, int boxCols)
 {

@@ -14,6 +14,10 @@ SELF_QUANTIZED = 2
 V2_IDENTITY_K1 = 4
 UNIQUE_ID_BYTES = 128
 PEER_HANDLE_BYTES = 64
+# element types, microscaled formats and pointwise functions of the mx_* calls
+F32, F16, BF16 = 0, 1, 2
+MXFP4, MXINT8 = 4, 8
+ACT_RELU, ACT_SIGMOID, ACT_TANH, ACT_GELU, ACT_SILU = 0, 1, 2, 3, 4
 
 EXPORTS = [
     "qagg_last_error", "qagg_abi_version", "qagg_packed_col_bytes", "qagg_packed_bytes", "qagg_stripe",
@@ -32,6 +36,8 @@ EXPORTS = [
     "qagg_sgd_update", "qagg_unquantize_sgd", "qagg_agg_bind_update", "qagg_agg_set_update", "qagg_agg_clear_status",
     "qagg_agg_f64_create", "qagg_agg_f64_step", "qagg_agg_f64_step_group", "qagg_agg_f64_reset_residuals", "qagg_agg_f64_residuals",
     "qagg_agg_f64_destroy", "qagg_agg_f64_copy_residual", "qagg_dense_set_fp16",
+    "qagg_mx_code_bytes", "qagg_mx_scale_bytes", "qagg_mx_quantize", "qagg_mx_unquantize", "qagg_mx_times", "qagg_mx_weight_grad", "qagg_mx_input_grad",
+    "qagg_mx_act_forward", "qagg_mx_act_backward", "qagg_mx_check",
 ]
 
 
@@ -139,6 +145,18 @@ _lib.qagg_hagg_destroy.argtypes = [c_vp]
 _lib.qagg_agg_set_profiling.argtypes = [c_vp, c_int]
 _lib.qagg_agg_phase_ms.argtypes = [c_vp, ctypes.POINTER(ctypes.c_float)]
 _lib.qagg_agg_destroy.argtypes = [c_vp]
+_lib.qagg_mx_code_bytes.restype = c_i64
+_lib.qagg_mx_code_bytes.argtypes = [c_i64, c_i64, c_int]
+_lib.qagg_mx_scale_bytes.restype = c_i64
+_lib.qagg_mx_scale_bytes.argtypes = [c_i64, c_i64]
+_lib.qagg_mx_quantize.argtypes = [c_vp, c_vp, c_int, c_i64, c_vp, c_vp, c_i64, c_i64, c_int, c_int]
+_lib.qagg_mx_unquantize.argtypes = [c_vp, c_vp, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_int]
+_lib.qagg_mx_times.argtypes = [c_vp] * 7 + [c_int] + [c_i64] * 4
+_lib.qagg_mx_weight_grad.argtypes = [c_vp, c_vp, c_int, c_i64, c_vp, c_vp, c_int, c_vp, c_i64, c_i64, c_i64, c_int]
+_lib.qagg_mx_input_grad.argtypes = [c_vp, c_vp, c_int, c_i64, c_vp, c_vp, c_int, c_vp, c_int, c_i64, c_i64, c_i64, c_i64]
+_lib.qagg_mx_act_forward.argtypes = [c_vp, c_vp, c_int, c_i64, c_int, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64]
+_lib.qagg_mx_act_backward.argtypes = [c_vp, c_vp, c_int, c_i64, c_vp, c_vp, c_int, c_vp, c_i64, c_i64, c_i64]
+_lib.qagg_mx_check.argtypes = [c_vp]
 
 
 def raw():
@@ -232,6 +250,59 @@ def quantize_to_host(grad_ptr, res_in_ptr, res_out_ptr, dev_scratch_ptr, host_pa
 
 def unquantize_from_host(host_packed_ptr, dev_scratch_ptr, out_ptr, M, N, bits, add=False, stream=0):
     _ok(_lib.qagg_unquantize_from_host(stream, host_packed_ptr, dev_scratch_ptr, out_ptr, M, N, bits, int(bool(add))))
+
+
+def mx_code_bytes(M, N, fmt):
+    v = _lib.qagg_mx_code_bytes(M, N, fmt)
+    if v < 0:
+        _ok(int(v))
+    return int(v)
+
+
+def mx_scale_bytes(M, N):
+    v = _lib.qagg_mx_scale_bytes(M, N)
+    if v < 0:
+        _ok(int(v))
+    return int(v)
+
+
+def mx_quantize(x_ptr, dtype, ld, codes_ptr, scales_ptr, M, N, fmt, transpose=False, stream=0):
+    """Microscaled form of an M x N matrix, or of its transpose (blocks along the columns)."""
+    _ok(_lib.qagg_mx_quantize(stream, x_ptr, dtype, ld, codes_ptr, scales_ptr, M, N, fmt, int(bool(transpose))))
+
+
+def mx_unquantize(codes_ptr, scales_ptr, out_ptr, dtype, ld, M, N, fmt, stream=0):
+    _ok(_lib.qagg_mx_unquantize(stream, codes_ptr, scales_ptr, out_ptr, dtype, ld, M, N, fmt))
+
+
+def mx_times(w_codes_ptr, w_scales_ptr, x_codes_ptr, x_scales_ptr, bias_ptr, y_ptr, y_dtype, ld_y, O, T, K, stream=0):
+    """y (O x T) = W x + bias, both operands 4-bit microscaled matrices of K rows; bias_ptr 0 or None: no bias."""
+    _ok(_lib.qagg_mx_times(stream, w_codes_ptr, w_scales_ptr, x_codes_ptr, x_scales_ptr, bias_ptr, y_ptr, y_dtype, ld_y, O, T, K))
+
+
+def mx_weight_grad(dy_ptr, dy_dtype, ld_dy, x_codes_ptr, x_scales_ptr, fmt, dw_ptr, O, I, T, add=False, stream=0):
+    """dw (O x I, fp32, the aggregator's layout) = or += dy (O x T) times the transpose of the packed x (I x T)."""
+    _ok(_lib.qagg_mx_weight_grad(stream, dy_ptr, dy_dtype, ld_dy, x_codes_ptr, x_scales_ptr, fmt, dw_ptr, O, I, T, int(bool(add))))
+
+
+def mx_input_grad(dy_ptr, dy_dtype, ld_dy, w_codes_ptr, w_scales_ptr, fmt, dx_ptr, dx_dtype, ld_dx, O, I, T, stream=0):
+    """dx (I x T) = packed w (I x O) times dy (O x T)."""
+    _ok(_lib.qagg_mx_input_grad(stream, dy_ptr, dy_dtype, ld_dy, w_codes_ptr, w_scales_ptr, fmt, dx_ptr, dx_dtype, ld_dx, O, I, T))
+
+
+def mx_act_forward(x_ptr, dtype, ld_x, act, y_ptr, ld_y, codes_ptr, scales_ptr, M, N, stream=0):
+    """y = f(x), and x kept as an 8-bit microscaled matrix for mx_act_backward."""
+    _ok(_lib.qagg_mx_act_forward(stream, x_ptr, dtype, ld_x, act, y_ptr, ld_y, codes_ptr, scales_ptr, M, N))
+
+
+def mx_act_backward(dy_ptr, dtype, ld_dy, codes_ptr, scales_ptr, act, dx_ptr, ld_dx, M, N, stream=0):
+    """dx = dy * f'(x as kept)."""
+    _ok(_lib.qagg_mx_act_backward(stream, dy_ptr, dtype, ld_dy, codes_ptr, scales_ptr, act, dx_ptr, ld_dx, M, N))
+
+
+def mx_check(stream=0):
+    """Waits for the stream and raises if a bounded wait inside a product kernel ran out since the last call."""
+    _ok(_lib.qagg_mx_check(stream))
 
 
 class Plan:

@@ -353,6 +353,69 @@ int qagg_stream_wait_selftest(void* stream, int max_tries, unsigned* status_dev,
  * polls have passed; on give-up it ORs 1 into *status_dev.  Never hangs. */
 int qagg_wait_flags(void* stream, const unsigned* flags_dev, int n, int skip, unsigned value, long long max_polls, unsigned* status_dev);
 
+/* ---- microscaled matrices: 4-bit products, 8-bit activation checkpoints ---------------------------------------------------
+ * What a data-parallel trainer holds and multiplies in few bits, next to what it sends in few bits.  No reference counterpart.
+ *
+ * Form.  An M x N matrix has blocks of 32 rows in each column (the last one padded with zeros).  A block shares the scale 2^X,
+ * stored as the byte X + 127, and its values are element * 2^X:
+ *   QAGG_MXFP4   4 bits: 0, .5, 1, 1.5, 2, 3, 4, 6 as codes 0..7, + 8 for the sign; two to a byte, the even row in the low half
+ *   QAGG_MXINT8  8 bits: q / 64, q = -127..127 in two's complement
+ * With a = the block's largest magnitude X = floor(log2 a) - 2 (fp4) or floor(log2 a) (int8), at least -127; elements are
+ * rounded to nearest, ties to even, and held at the largest one (6, 127/64).  A block of zeros has byte 0.  A block that holds a
+ * NaN or an infinity has byte 255 and codes 0: all of its values are NaN.
+ * Codes: column after column, qagg_mx_code_bytes(M, 1, format) bytes each (whole blocks).  Scales: bytes in tiles of 128 columns x
+ * 4 blocks, 512 bytes each, the tiles of one 128 columns one after the other; in a tile the byte of column j and block b is at
+ * (j % 32) * 16 + (j % 128 / 32) * 4 + b % 4, and missing columns and blocks have byte 0.  Both arrays must be 16-byte aligned;
+ * the quantizing calls write all qagg_mx_code_bytes() / qagg_mx_scale_bytes() bytes of them.
+ *
+ * Dense matrices are column-major with `ld` elements from one column to the next (ld >= rows), of type QAGG_F32, QAGG_F16 or
+ * QAGG_BF16, aligned to their type.  bf16 operands whose base and ld are multiples of 16 bytes are the fast case of the products;
+ * any other alignment, and fp16 and fp32, are taken too.  Results do not depend on alignment.  Elements between a column's
+ * rows and its ld are neither read nor written.  Rows < 2^30, columns <= 65535 * 128 (the second dimension of a gradient product's
+ * result: 65535 * 64).  Sums and functions are computed in fp32 and rounded once to the output type.  All calls only enqueue
+ * kernels on `stream` (they may be captured), allocate nothing and use no workspace: calls on different streams are independent.
+ * As everywhere in this library the buffers and the stream belong to the current device. */
+#define QAGG_F32 0
+#define QAGG_F16 1
+#define QAGG_BF16 2
+#define QAGG_MXFP4 4
+#define QAGG_MXINT8 8
+int64_t qagg_mx_code_bytes(int64_t M, int64_t N, int format);
+int64_t qagg_mx_scale_bytes(int64_t M, int64_t N);
+/* x (M x N) -> packed.  transpose == 0: the packed matrix is x, M x N.  Otherwise it is the transpose, N x M: its blocks run along
+ * the columns of x.  A weight O x K becomes an operand of qagg_mx_times that way. */
+int qagg_mx_quantize(void* stream, const void* x, int type, int64_t ld, void* codes, void* scales, int64_t M, int64_t N, int format, int transpose);
+/* packed M x N -> values. */
+int qagg_mx_unquantize(void* stream, const void* codes, const void* scales, void* out, int type, int64_t ld, int64_t M, int64_t N, int format);
+/* y = Times(W, x) + bias: y (O x T), y(o, t) = sum over k < K of w(k, o) * x(k, t) + bias(o), both operands packed QAGG_MXFP4 matrices
+ * of K rows (w: the transpose of the O x K weight).  bias: O floats or NULL.  K == 0 gives the bias alone.  T == 1 is the
+ * single-token form. */
+int qagg_mx_times(void* stream, const void* w_codes, const void* w_scales, const void* x_codes, const void* x_scales, const float* bias, void* y, int y_type, int64_t ld_y,
+                  int64_t O, int64_t T, int64_t K);
+/* The backward pass of a layer y = W x (rounding is passed through: gradients are those at the packed operands' values).
+ * weight_grad: dw (O x I, fp32, no gaps: what qagg_agg_step takes) = sum over t of dy(o, t) * x(i, t), x packed I x T in either
+ *   format; add != 0 adds to what dw holds (several minibatches before one aggregation).
+ * input_grad: dx (I x T) = sum over o of w(i, o) * dy(o, t), w packed I x O in either format, as qagg_mx_times takes it.
+ * dy is O x T.  The packed values are exact in the product; fp16 and fp32 dy are taken as exact sums of two and three bf16 terms
+ * (magnitudes below about 2^-109 lose their last bits). */
+int qagg_mx_weight_grad(void* stream, const void* dy, int dy_type, int64_t ld_dy, const void* x_codes, const void* x_scales, int format, float* dw, int64_t O, int64_t I,
+                        int64_t T, int add);
+int qagg_mx_input_grad(void* stream, const void* dy, int dy_type, int64_t ld_dy, const void* w_codes, const void* w_scales, int format, void* dx, int dx_type, int64_t ld_dx,
+                       int64_t O, int64_t I, int64_t T);
+/* Pointwise layers whose input is kept in 8 bits: forward writes y = f(x) and x as a packed QAGG_MXINT8 matrix, backward
+ * dx = dy * f'(x as kept).  y may be x, dx may be dy (same ld).  QAGG_ACT_GELU is x * Phi(x), QAGG_ACT_SILU x * sigmoid(x); the slope of
+ * QAGG_ACT_RELU at 0 (also at values that were rounded to 0) is 0.  A kept block with a NaN or an infinity gives NaN gradients. */
+#define QAGG_ACT_RELU 0
+#define QAGG_ACT_SIGMOID 1
+#define QAGG_ACT_TANH 2
+#define QAGG_ACT_GELU 3
+#define QAGG_ACT_SILU 4
+int qagg_mx_act_forward(void* stream, const void* x, int type, int64_t ld_x, int act, void* y, int64_t ld_y, void* codes, void* scales, int64_t M, int64_t N);
+int qagg_mx_act_backward(void* stream, const void* dy, int type, int64_t ld_dy, const void* codes, const void* scales, int act, void* dx, int64_t ld_dx, int64_t M, int64_t N);
+/* Waits for `stream`; QAGG_ETIMEOUT if a bounded wait inside a product kernel ran out since the last call (never observed), and
+ * clears that report. */
+int qagg_mx_check(void* stream);
+
 /* Per-phase device timing of the steps that follow (no reference counterpart; the reference only has the wall-clock
  * "Actual gradient aggregation time" trace, AllReduceDistGradAggregator.h:241-246, 560-565).  When enabled, each step records
  * CUDA events on its stream around its five phases.  qagg_agg_phase_ms waits for the recorded steps and returns the mean
