@@ -233,9 +233,9 @@ cudaError_t launch_materialize(cudaStream_t st, const float* buf, const float* l
 
 // error plumbing (qagg_capi.cu)
 // tensor map (64-byte aligned, 128 bytes) of `outer` rows of `inner` contiguous bf16 values (elemBytes 2) or bytes (1), rows strideBytes
-// apart; reads outside give zero.  base 16-byte aligned, strideBytes a multiple of 16.
+// apart; reads outside give zero.  swizzle: span in bytes, 128, 64 or 0 (none).  base 16-byte aligned, strideBytes a multiple of 16.
 bool encode_map_tiled(void* out128, int elemBytes, const void* base, long long inner, long long outer, long long strideBytes, int boxInner, int boxOuter,
-                      bool swizzle128);
+                      int swizzle);
 int fail(int code, const std::string& msg);
 int check_cuda(cudaError_t e, const char* what);
 bool bits_ok(int bits);

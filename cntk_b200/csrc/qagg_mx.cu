@@ -18,24 +18,6 @@ constexpr int MX_PASSES = MX_TILE / MX_PASS;
 
 // ---- eight values of one column -------------------------------------------------------------------------------------------
 
-template <class T>
-struct Raw8;
-template <>
-struct Raw8<float>
-{
-    uint4 a, b;
-};
-template <>
-struct Raw8<__half>
-{
-    uint4 a;
-};
-template <>
-struct Raw8<__nv_bfloat16>
-{
-    uint4 a;
-};
-
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -48,28 +30,6 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// n = values that exist (0..8); the others read as zero.  vec: the address is 16-byte aligned.
-template <class T>
-__device__ __forceinline__ Raw8<T> load8(const T* p, int n, bool vec)
-{
-    Raw8<T> r = {};
-    if (vec && n == 8)
-    {
-        const uint4* q = reinterpret_cast<const uint4*>(p);
-        r.a = __ldcs(q);
-        if constexpr (sizeof(T) == 4)
-            r.b = __ldcs(q + 1);
-    }
-    else
-    {
-        T* e = reinterpret_cast<T*>(&r);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < n)
-                e[i] = p[i];
-    }
-    return r;
-}
 template <class T>
 __device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&v)[8])
 {

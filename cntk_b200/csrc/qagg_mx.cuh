@@ -49,6 +49,47 @@ __device__ __forceinline__ float mx_scale_inv(unsigned byte)
     return __uint_as_float(byte < 254u ? (254u - byte) << 23 : 0x00400000u);
 }
 
+// eight values of one column as they were loaded
+template <class T>
+struct Raw8;
+template <>
+struct Raw8<float>
+{
+    uint4 a, b;
+};
+template <>
+struct Raw8<__half>
+{
+    uint4 a;
+};
+template <>
+struct Raw8<__nv_bfloat16>
+{
+    uint4 a;
+};
+
+// n = values that exist (0..8); the others read as zero.  vec: the address is 16-byte aligned.
+template <class T>
+__device__ __forceinline__ Raw8<T> load8(const T* p, int n, bool vec)
+{
+    Raw8<T> r = {};
+    if (vec && n == 8)
+    {
+        const uint4* q = reinterpret_cast<const uint4*>(p);
+        r.a = __ldcs(q);
+        if constexpr (sizeof(T) == 4)
+            r.b = __ldcs(q + 1);
+    }
+    else
+    {
+        T* e = reinterpret_cast<T*>(&r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n)
+                e[i] = p[i];
+    }
+    return r;
+}
 // argument checks shared by the entry points (host)
 int mx_check_dims(const char* who, long long M, long long N);
 bool mx_type_ok(int type);

@@ -6,9 +6,18 @@
 //               dense.  The packed operand's blocks run across the contraction, so its scales cannot go with a block-scaled
 //               product; it is expanded to bf16 (exact) on the way, straight into tensor memory, as operand A.
 //
-// Both: one CTA per 128 x n output tile; a copy warp feeds a ring of shared-memory stages, one thread issues the products, eight
-// warps take the result from tensor memory.  Where there are fewer tiles than SMs the contraction is split over the CTAs of a cluster,
-// whose partial sums are added through distributed shared memory in rank order: no workspace, no atomics, the same bits on every run.
+// Both: 128 x n output tiles, dealt to one resident CTA per SM.  A copy warp feeds a ring of shared-memory stages and runs ahead into
+// the next tile, one thread issues the products, eight (or four) result warps hold the tile's sums in registers.
+//
+// The sums.  The tensor cores add to their fp32 accumulator with truncation: sums of n instructions come out low by up to n / 2 units in
+// the last place, 6.8e-6 of the result after 512 of them.  So where the output is fp32 a chain ends after CHAIN instructions; the
+// result warps add its value to their registers (round to nearest) and hand the accumulator back, which takes about 2000 cycles
+// from the last product to the next.  Two accumulators in turn hide that, and the next tile begins while this one is being
+// written.  (A 256-wide tile of the 4-bit product has room for one.)  For 16-bit outputs, which round 300 times more coarsely, a
+// chain is CHAIN_16BIT instructions.
+//
+// Where there are fewer tiles than SMs the contraction is split over the CTAs of a cluster, whose partial sums are added through
+// distributed shared memory in rank order: no workspace, no atomics, the same bits on every run.
 #include "qagg_mx.cuh"
 #include "qagg_tcgen05.cuh"
 
@@ -21,172 +30,266 @@ namespace qagg {
 // set by a bounded wait that ran out; read and cleared by qagg_mx_check
 __device__ unsigned g_mxStatus;
 
-constexpr int GT = 384;            // threads: copy warp, product warp, allocating warp, spare, eight result warps
-constexpr int GT_DENSE = 640;      // and eight warps that bring a dense operand which the copy engine cannot take
-constexpr unsigned TMEM_COLS = 512;
+constexpr unsigned TMEM_COLS = 512; // accumulators first; behind them block scales or expanded operands
 constexpr int MAX_STAGES = 8;
-constexpr int GEMM_SMEM_MAX = 224 * 1024; // dynamic; barriers and scale pairs take a little more
+constexpr int GEMM_SMEM_MAX = 224 * 1024; // dynamic; barriers and scales take a little more
 // More than half of an SM's shared memory, always: a second CTA on the SM would wait for tensor memory (all columns are taken),
 // and CTAs of two clusters that each wait for the other's tensor memory would never meet at their cluster barriers.
 constexpr int GEMM_SMEM_MIN = 118 * 1024;
+// tensor-core instructions in a row on one accumulator: their truncation stays near 5e-7 of the sum
+constexpr int CHAIN = 32, CHAIN_16BIT = 1024;
 
 struct GemmBars
 {
     unsigned long long full[MAX_STAGES];  // copies of the stage have landed
-    unsigned long long conv[MAX_STAGES];  // grad: packed operand expanded into tensor memory
-    unsigned long long dense[MAX_STAGES]; // grad, dense loaders: their part of the stage is written
+    unsigned long long conv[MAX_STAGES];  // gradients: packed operand expanded into tensor memory
+    unsigned long long dense[MAX_STAGES]; // gradients, dense loaders: their part of the stage is written
     unsigned long long empty[MAX_STAGES]; // products that read the stage are done
-    unsigned long long done;              // all products are done
+    unsigned long long ready[2];          // the accumulator holds a finished chain
+    unsigned long long taken[2];          // the result warps have it
     unsigned tmem;
     unsigned broken;
 };
 
-__device__ __forceinline__ void put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+// place in the ring of stages and the parity of its current round
+struct Ring
+{
+    int s = 0;
+    unsigned par = 0;
+    __device__ __forceinline__ void next(int stages)
+    {
+        if (++s == stages)
+        {
+            s = 0;
+            par ^= 1;
+        }
+    }
+};
 
-// First and last-but-one step of this CTA's part of the contraction.
+// this CTA's steps of the contraction
 __device__ __forceinline__ void split_range(int steps, int rank, int splits, int& first, int& count)
 {
     first = (int) ((long long) steps * rank / splits);
     count = (int) ((long long) steps * (rank + 1) / splits) - first;
 }
 
-// ---- results ------------------------------------------------------------------------------------------------------------------
-// The tile D (128 lanes m x bn columns n) goes out as
-//   columns  out[(n0 + n) * ld + m0 + m], any type: 32 lanes are 32 neighbours, so straight from the registers
-//   rows     out[(m0 + m) * ld + n0 + n], fp32: through shared memory, whose rows are then written 16 values a thread apart
-// Eight warps (`warp` 0..7 of them): lanes 32 * (warp % 4), 32-column pieces alternating between warp / 4 = 0, 1.
-template <bool ROWS, class T>
-__device__ __forceinline__ void write_tile(unsigned tmemD, bool zero, int bn, int warp, float* buf, int splits, int rank, T* out, long long ld, long long m0,
-                                           long long M, long long n0, long long N, const float* bias, bool add)
-{
-    const int lane = threadIdx.x & 31, quad = warp & 3;
-    const int m = quad * 32 + lane;
-    const int pitch = ROWS ? bn + 4 : 128; // ROWS: [m][n], else [n][m]
-    const bool viaShared = ROWS || splits > 1;
-    if (warp >= 0)
-    {
-        const float b = bias && m0 + m < M && splits == 1 ? bias[m0 + m] : 0.0f;
-        for (int c = (warp >> 2) * 32; c < bn; c += 64)
-        {
-            unsigned r[32];
-            if (zero)
-            {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    r[j] = 0;
-            }
-            else
-                tmem_load32(tmemD + ((unsigned) (quad * 32) << 16) + c, r);
-            if (viaShared)
-            {
-                if (ROWS)
-                {
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        *reinterpret_cast<uint4*>(buf + m * pitch + c + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
-                }
-                else
-                {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (c + j < bn)
-                            buf[(c + j) * pitch + m] = __uint_as_float(r[j]);
-                }
-            }
-            else if (m0 + m < M)
-            {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    if (c + j < bn && n0 + c + j < N)
-                        put(out + (n0 + c + j) * ld + m0 + m, __uint_as_float(r[j]) + b);
-            }
-        }
-    }
-    if (!viaShared)
-        return;
-    __syncwarp();
-    if (splits > 1)
-        cluster_sync();
-    else
-        __syncthreads();
-    // this CTA's share of the tile: rows (ROWS) or columns, four values a time
-    const int lines = ROWS ? 128 : bn, width = ROWS ? bn : 128;
-    const int l0 = lines * rank / splits, l1 = lines * (rank + 1) / splits;
-    const unsigned base = smem_addr(buf);
-    if (warp >= 0)
-    {
-        const int perLine = width / 4;
-        for (int u = l0 * perLine + warp * 32 + lane; u < l1 * perLine; u += 256)
-        {
-            const int l = u / perLine, w = (u - l * perLine) * 4;
-            const unsigned at = base + (unsigned) (l * pitch + w) * 4;
-            float4 s = *reinterpret_cast<const float4*>(buf + l * pitch + w);
-            if (splits > 1)
-            {
-                s = cluster_load4(at, 0);
-                for (int k = 1; k < splits; ++k)
-                {
-                    const float4 v = cluster_load4(at, k);
-                    s.x += v.x;
-                    s.y += v.y;
-                    s.z += v.z;
-                    s.w += v.w;
-                }
-            }
-            const float e[4] = {s.x, s.y, s.z, s.w};
-            const long long line = (ROWS ? m0 : n0) + l, col = (ROWS ? n0 : m0) + w;
-            const long long nl = ROWS ? M : N, nc = ROWS ? N : M;
-            if (line >= nl)
-                continue;
-            T* p = out + line * ld + col;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (col + j < nc)
-                {
-                    if constexpr (ROWS)
-                        p[j] = add ? p[j] + e[j] : e[j];
-                    else
-                        put(p + j, e[j] + (bias ? bias[col + j] : 0.0f));
-                }
-        }
-    }
-    __syncwarp();
-    if (splits > 1)
-        cluster_sync(); // nobody leaves while its partial sums are being read
-}
-
 // After a wait ran out: the copies this thread started have landed (or a bounded wait for them ran out too) before the CTA goes.
-__device__ __forceinline__ void drain_copies(GemmBars* bars, int issued, int stages)
+__device__ __forceinline__ void drain_copies(GemmBars* bars, long long issued, int stages)
 {
     const unsigned long long began = clock_ns();
-    for (int i = issued > stages ? issued - stages : 0; i < issued; ++i)
-        while (!mbar_suspend_wait(&bars->full[i % stages], (i / stages) & 1) && clock_ns() - began < TC_WAIT_NS)
+    for (long long i = issued > stages ? issued - stages : 0; i < issued; ++i)
+        while (!mbar_suspend_wait(&bars->full[i % stages], (unsigned) (i / stages) & 1) && clock_ns() - began < TC_WAIT_NS)
             ;
 }
 
-__device__ __forceinline__ void gemm_setup(GemmBars* bars, int stages, int convCount, int denseCount)
+// First warp: barriers.  The copies may start right after this, before the CTA has met.
+__device__ __forceinline__ void init_barriers(GemmBars* bars, int stages, int convCount, int denseCount, int resultWarps)
 {
-    if (threadIdx.x == 0)
+    for (int s = 0; s < stages; ++s)
     {
-        for (int s = 0; s < stages; ++s)
-        {
-            mbar_init(&bars->full[s], 1);
-            mbar_init(&bars->conv[s], convCount);
-            mbar_init(&bars->dense[s], denseCount);
-            mbar_init(&bars->empty[s], 1);
-        }
-        mbar_init(&bars->done, 1);
-        bars->broken = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        fence_async_shared();
+        mbar_init(&bars->full[s], 1);
+        mbar_init(&bars->conv[s], convCount);
+        mbar_init(&bars->dense[s], denseCount);
+        mbar_init(&bars->empty[s], 1);
     }
-    if (threadIdx.x >> 5 == 2)
-        tmem_alloc(&bars->tmem, TMEM_COLS);
-    tc_fence_before();
-    __syncthreads();
+    for (int b = 0; b < 2; ++b)
+    {
+        mbar_init(&bars->ready[b], 1);
+        mbar_init(&bars->taken[b], resultWarps);
+    }
+    bars->broken = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_shared();
+}
+
+// ---- results ------------------------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ unsigned pack2(float a, float b, __half*)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const unsigned*>(&h);
+}
+__device__ __forceinline__ unsigned pack2(float a, float b, __nv_bfloat16*)
+{
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const unsigned*>(&h);
+}
+
+// `cols` columns (a multiple of 16) of a finished chain, set or added to the registers.
+template <int ACC>
+__device__ __forceinline__ void take_chain(GemmBars* bars, int buf, unsigned par, unsigned tmem, int cols, bool firstChain, float (&acc)[ACC])
+{
+    tc_wait(&bars->ready[buf], par, &bars->broken, &g_mxStatus);
+    __syncwarp();
     tc_fence_after();
+#pragma unroll
+    for (int p = 0; p < ACC / 16; ++p)
+        if (p * 16 < cols)
+        {
+            unsigned r[16];
+            tmem_load16(tmem + p * 16, r);
+            tmem_load_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                acc[p * 16 + j] = firstChain ? __uint_as_float(r[j]) : acc[p * 16 + j] + __uint_as_float(r[j]);
+        }
+    tc_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0)
+        mbar_arrive(&bars->taken[buf]);
+}
+// Which accumulator a chain uses, and the parity of its barriers' phase.
+struct Chains
+{
+    int buf = 0;
+    unsigned par = 0;
+    __device__ __forceinline__ void next(int bufs)
+    {
+        if (++buf >= bufs)
+        {
+            buf = 0;
+            par ^= 1;
+        }
+    }
+};
+
+// Sums of one lane (row m of the tile) and `cols` columns from n on, straight to the output:
+//   columns  out[n * ld + m]: 32 lanes are 32 neighbours (`partner`: the lane whose row is m ^ 1; 16-bit types are stored in pairs)
+//   rows     out[m * ld + n], fp32: 16 bytes a thread where the alignment allows
+template <class T, int ACC>
+__device__ __forceinline__ void write_columns(T* out, long long ld, long long m, long long M, long long n, long long N, int cols, const float (&acc)[ACC], float bias,
+                                              int partner, bool pairs)
+{
+    const long long left = N - n;
+    const int c = (int) (left < cols ? left : cols);
+    if constexpr (sizeof(T) == 2)
+    {
+        if (pairs) // uniform: all rows of the tile exist, ld is even, the base 4-byte aligned
+        {
+            const bool odd = m & 1;
+            T* p = out + (n + odd) * ld + (m & ~1LL);
+            const long long two = 2 * ld;
+#pragma unroll
+            for (int j = 0; j < ACC; j += 2)
+            {
+                // this lane stores column j (even row) or j + 1 (odd row) of its pair of rows
+                const float a = acc[j] + bias, b = acc[j + 1] + bias;
+                const float got = __shfl_sync(0xffffffffu, odd ? a : b, partner);
+                const unsigned v = odd ? pack2(got, b, (T*) nullptr) : pack2(a, got, (T*) nullptr);
+                if (j + (odd ? 1 : 0) < c)
+                    *reinterpret_cast<unsigned*>(p) = v;
+                p += two;
+            }
+            return;
+        }
+    }
+    if (m >= M)
+        return;
+    T* p = out + n * ld + m;
+#pragma unroll
+    for (int j = 0; j < ACC; ++j)
+    {
+        if (j < c)
+            put(p, acc[j] + bias);
+        p += ld;
+    }
+}
+template <int ACC>
+__device__ __forceinline__ void write_row(float* out, long long ld, long long m, long long M, long long n, long long N, int cols, const float (&acc)[ACC], bool add, bool vec)
+{
+    if (m >= M)
+        return;
+    const long long left = N - n;
+    const int c = (int) (left < cols ? left : cols);
+    float* p = out + m * ld + n;
+#pragma unroll
+    for (int j = 0; j < ACC; j += 4)
+    {
+        if (vec && j + 4 <= c)
+        {
+            float4* q = reinterpret_cast<float4*>(p + j);
+            float4 v = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+            if (add)
+            {
+                const float4 o = *q;
+                v = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+            }
+            *q = v;
+        }
+        else
+        {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (j + e < c)
+                    p[j + e] = add ? p[j + e] + acc[j + e] : acc[j + e];
+        }
+    }
+}
+
+// Split contraction: each CTA leaves its partial sums in its shared memory ([n][128 rows], or for rows [m][bn + 4]), and CTA `rank` adds
+// up and writes its share of the tile's columns (rows).  Called by all threads; result warps have put their sums down.
+template <bool ROWS, class T>
+__device__ __forceinline__ void reduce_cluster(float* buf, int splits, int rank, int bn, T* out, long long ld, long long m0, long long M, long long n0, long long N,
+                                               const float* bias, bool add)
+{
+    __syncwarp();
+    cluster_sync();
+    const long long restM = M - m0, restN = N - n0;
+    const int rows = (int) (restM < 128 ? restM : 128), cols = (int) (restN < bn ? restN : bn);
+    const int pitch = ROWS ? bn + 4 : 128;
+    const int lines = ROWS ? rows : cols, width = ROWS ? cols : rows;
+    const int perLine = (width + 3) / 4;
+    const int u1 = (int) ((long long) lines * perLine * (rank + 1) / splits);
+    for (int u = (int) ((long long) lines * perLine * rank / splits) + (int) threadIdx.x; u < u1; u += blockDim.x)
+    {
+        const int l = u / perLine, w = (u - l * perLine) * 4;
+        const unsigned at = smem_addr(buf + l * pitch + w);
+        float4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < splits)
+                v[k] = cluster_load4(cluster_address(at, k));
+        float4 s = v[0];
+#pragma unroll
+        for (int k = 1; k < 8; ++k)
+            if (k < splits)
+                s = make_float4(s.x + v[k].x, s.y + v[k].y, s.z + v[k].z, s.w + v[k].w);
+        const float e[4] = {s.x, s.y, s.z, s.w};
+        const long long col = (ROWS ? n0 : m0) + w;
+        T* p = out + ((ROWS ? m0 : n0) + l) * ld + col;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (w + j < width)
+            {
+                if constexpr (ROWS)
+                    p[j] = add ? p[j] + e[j] : e[j];
+                else
+                    put(p + j, e[j] + (bias ? bias[col + j] : 0.0f));
+            }
+    }
+    __syncwarp();
+    cluster_sync(); // nobody leaves while its partial sums are being read
+}
+template <bool ROWS, int ACC>
+__device__ __forceinline__ void put_partial(float* buf, int bn, int m, int col0, int cols, const float (&acc)[ACC])
+{
+    if constexpr (ROWS)
+    {
+#pragma unroll
+        for (int j = 0; j < ACC; j += 4)
+            if (j < cols)
+                *reinterpret_cast<float4*>(buf + m * (bn + 4) + col0 + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+    }
+    else
+    {
+#pragma unroll
+        for (int j = 0; j < ACC; ++j)
+            if (j < cols)
+                buf[(col0 + j) * 128 + m] = acc[j];
+    }
 }
 
 // ---- 4-bit product --------------------------------------------------------------------------------------------------------------
@@ -198,10 +301,12 @@ struct TimesArgs
     const float* bias;
     void* y;
     long long ld, O, T, K;
-    int bn, stages, splits;
+    int bn, stages, splits, tilesM, tiles, pairs;
 };
 
-constexpr int TK = 256; // contraction values per stage: 128 bytes of codes
+constexpr int TT = 384;  // copy, product, allocating and spare warp; eight result warps
+constexpr int TK = 256;  // contraction values per stage: 128 bytes of codes
+
 
 __host__ __device__ inline int times_stage_bytes(int bn)
 {
@@ -209,80 +314,169 @@ __host__ __device__ inline int times_stage_bytes(int bn)
 }
 
 template <class T>
-__global__ void __launch_bounds__(GT, 1) k_mx_times(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapX, const TimesArgs a)
+__global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapX, const TimesArgs a)
 {
     extern __shared__ unsigned char dyn[];
     __shared__ GemmBars bars;
     unsigned char* stage0 = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t) 1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int bn = a.bn, S = a.stages, stageBytes = times_stage_bytes(bn);
-    const long long m0 = (long long) blockIdx.x * 128, n0 = (long long) blockIdx.y * bn;
     const int steps = (int) ((a.K + TK - 1) / TK);
     const int rank = a.splits > 1 ? (int) cluster_rank() : 0;
     int first, count;
     split_range(steps, rank, a.splits, first, count);
     const long long chunks = mx_scale_tiles(a.K); // scale tiles along the contraction, 128 values each
-    const int rowsX = bn > 128 && n0 + 128 < a.T ? 2 : 1;
+    const int resultWarps = bn > 128 ? 8 : 4;
+    const int bufs = bn > 128 ? 1 : 2; // accumulators, 128 columns apart
+    constexpr unsigned SIDE = 256;     // block scales: 24 columns a stage
+    constexpr int CHAIN_STEPS = (sizeof(T) == 4 ? CHAIN : CHAIN_16BIT) / 4;
 
-    gemm_setup(&bars, S, 1, 1);
-    const unsigned tm = bars.tmem;
-    const unsigned scales = tm + 256; // 24 columns a stage: 8 of W, 16 of X
-    if (warp == 0 && lane == 0)
+    auto copy_step = [&](int tile, int i, int s) {
+        const long long m0 = (long long) (tile % a.tilesM) * 128, n0 = (long long) (tile / a.tilesM) * bn;
+        const int rowsX = bn > 128 && n0 + 128 < a.T ? 2 : 1;
+        const unsigned at = smem_addr(stage0) + s * stageBytes;
+        const int k = first + i;
+        const unsigned nch = chunks - 2LL * k < 2 ? 1 : 2;
+        mbar_arrive_expect_tx(&bars.full[s], 128 * 128 + bn * 128 + nch * 512 * (1 + rowsX));
+        tma_load_2d(at, &mapW, k * 128, (int) m0, &bars.full[s]);
+        tma_load_2d(at + 16384, &mapX, k * 128, (int) n0, &bars.full[s]);
+        const unsigned sw = at + 16384 + bn * 128;
+        bulk_load(sw, a.scaleW + ((m0 / 128) * chunks + 2LL * k) * 512, nch * 512, &bars.full[s]);
+        for (int r = 0; r < rowsX; ++r)
+            bulk_load(sw + 1024 + r * 1024, a.scaleX + ((n0 / 128 + r) * chunks + 2LL * k) * 512, nch * 512, &bars.full[s]);
+    };
+    int early = 0; // steps of the first tile whose copies start before the CTA has met
+    if (warp == 0)
     {
-        for (int i = 0; i < count; ++i)
+        if (elect_one())
         {
-            const int s = i % S;
-            if (i >= S)
-                tc_wait(&bars.empty[s], ((i / S) & 1) ^ 1, &bars.broken, &g_mxStatus);
-            if (*reinterpret_cast<volatile unsigned*>(&bars.broken))
-            {
-                drain_copies(&bars, i, S);
-                break;
-            }
-            const unsigned at = smem_addr(stage0 + (size_t) s * stageBytes);
-            const int k = first + i;
-            const unsigned nch = (unsigned) (chunks - 2LL * k < 2 ? 1 : 2);
-            mbar_arrive_expect_tx(&bars.full[s], 128 * 128 + bn * 128 + nch * 512 * (1 + rowsX));
-            tma_load_2d(at, &mapW, k * 128, (int) m0, &bars.full[s]);
-            tma_load_2d(at + 16384, &mapX, k * 128, (int) n0, &bars.full[s]);
-            const unsigned sw = at + 16384 + bn * 128;
-            bulk_load(sw, a.scaleW + ((m0 / 128) * chunks + 2LL * k) * 512, nch * 512, &bars.full[s]);
-            for (int r = 0; r < rowsX; ++r)
-                bulk_load(sw + 1024 + r * 1024, a.scaleX + ((n0 / 128 + r) * chunks + 2LL * k) * 512, nch * 512, &bars.full[s]);
+            init_barriers(&bars, S, 1, 1, resultWarps);
+            for (; early < count && early < S; ++early)
+                copy_step(blockIdx.x, early, early);
         }
+        early = count < S ? count : S;
+        __syncwarp();
     }
-    else if (warp == 1 && lane == 0)
-    {
-        for (int i = 0; i < count; ++i)
-        {
-            const int s = i % S;
-            tc_wait(&bars.full[s], (i / S) & 1, &bars.broken, &g_mxStatus);
-            tc_fence_after();
-            const unsigned at = smem_addr(stage0 + (size_t) s * stageBytes);
-            const unsigned sw = at + 16384 + bn * 128;
-            const long long left = a.K - (long long) (first + i) * TK;
-            const int nch = left > 128 ? 2 : 1;
-            const int nk = left >= TK ? 4 : (int) ((left + 63) / 64);
-            const unsigned sa = scales + s * 24, sb = sa + 8;
-            for (int c = 0; c < nch; ++c)
-            {
-                tmem_copy_scales(sa + c * 4, smem_desc(sw + c * 512, 16, 128, SWIZZLE_NONE));
-                for (int r = 0; r < rowsX; ++r)
-                    tmem_copy_scales(sb + c * 8 + r * 4, smem_desc(sw + 1024 + r * 1024 + c * 512, 16, 128, SWIZZLE_NONE));
-            }
-            for (int j = 0; j < nk; ++j)
-                mma_mxf4_ss(tm, smem_desc(at + j * 32, 16, 1024, SWIZZLE_128B), smem_desc(at + 16384 + j * 32, 16, 1024, SWIZZLE_128B), idesc_mxf4(bn, (j & 1) * 2),
-                            sa + (j >> 1) * 4, sb + (j >> 1) * 8, i + j > 0);
-            tc_commit(&bars.empty[s]);
-        }
-        tc_commit(&bars.done);
-    }
-    __syncwarp();
-    // every thread sees the end of the products before shared memory is used again and tensor memory is given back
-    tc_wait(&bars.done, 0, &bars.broken, &g_mxStatus);
-    __syncwarp();
+    if (warp == 2)
+        tmem_alloc(&bars.tmem, TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
     tc_fence_after();
-    write_tile<false, T>(tm, count == 0, bn, warp - 4, reinterpret_cast<float*>(stage0), a.splits, rank, (T*) a.y, a.ld, m0, a.O, n0, a.T, a.bias, false);
+    const unsigned tm = bars.tmem;
+
+    if (warp == 0)
+    {
+        if (elect_one())
+        {
+            Ring ring;
+            for (int i = 0; i < early; ++i)
+                ring.next(S);
+            long long issued = early;
+            for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
+                for (int i = tile == (int) blockIdx.x ? early : 0; i < count; ++i, ++issued)
+                {
+                    if (issued >= S)
+                        tc_wait(&bars.empty[ring.s], ring.par ^ 1, &bars.broken, &g_mxStatus);
+                    if (*reinterpret_cast<volatile unsigned*>(&bars.broken))
+                    {
+                        drain_copies(&bars, issued, S);
+                        i = count;
+                        tile = a.tiles;
+                        break;
+                    }
+                    copy_step(tile, i, ring.s);
+                    ring.next(S);
+                }
+        }
+    }
+    else if (warp == 1)
+    {
+        if (elect_one())
+        {
+            Ring ring;
+            Chains chain;
+            bool fresh = true; // accumulators that no chain has used
+            const unsigned id0 = idesc_mxf4(bn, 0), id2 = idesc_mxf4(bn, 2);
+            const unsigned long long dW = smem_desc(smem_addr(stage0), 16, 1024, SWIZZLE_128B);
+            const unsigned long long dX = dW + (16384 >> 4);
+            const unsigned long long dS = smem_desc(smem_addr(stage0) + 16384 + bn * 128, 16, 128, SWIZZLE_NONE);
+            for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
+            {
+                const long long n0 = (long long) (tile / a.tilesM) * bn;
+                const bool twoX = bn > 128 && n0 + 128 < a.T;
+                int inChain = 0;
+                for (int i = 0; i < count; ++i)
+                {
+                    if (inChain == 0 && !fresh)
+                        tc_wait(&bars.taken[chain.buf], chain.par ^ 1, &bars.broken, &g_mxStatus);
+                    tc_wait(&bars.full[ring.s], ring.par, &bars.broken, &g_mxStatus);
+                    tc_fence_after();
+                    const unsigned d = tm + chain.buf * 128;
+                    const unsigned long long off = (unsigned long long) (unsigned) (ring.s * stageBytes) >> 4;
+                    const unsigned long long w = dW + off, x = dX + off, sc = dS + off;
+                    const unsigned sa = tm + SIDE + ring.s * 24, sb = sa + 8; // eight columns of W's scales, sixteen of X's
+                    const long long left = a.K - (long long) (first + i) * TK;
+                    const bool more = inChain > 0;
+                    tmem_copy_scales(sa, sc);
+                    tmem_copy_scales(sb, sc + (1024 >> 4));
+                    if (twoX)
+                        tmem_copy_scales(sb + 4, sc + (2048 >> 4));
+                    mma_mxf4_ss(d, w, x, id0, sa, sb, more);
+                    if (left > 64)
+                        mma_mxf4_ss(d, w + 2, x + 2, id2, sa, sb, true);
+                    if (left > 128)
+                    {
+                        tmem_copy_scales(sa + 4, sc + (512 >> 4));
+                        tmem_copy_scales(sb + 8, sc + (1536 >> 4));
+                        if (twoX)
+                            tmem_copy_scales(sb + 12, sc + (2560 >> 4));
+                        mma_mxf4_ss(d, w + 4, x + 4, id0, sa + 4, sb + 8, true);
+                        if (left > 192)
+                            mma_mxf4_ss(d, w + 6, x + 6, id2, sa + 4, sb + 8, true);
+                    }
+                    tc_commit(&bars.empty[ring.s]);
+                    ring.next(S);
+                    if (++inChain == CHAIN_STEPS || i + 1 == count)
+                    {
+                        tc_commit(&bars.ready[chain.buf]);
+                        chain.next(bufs);
+                        fresh = fresh && chain.buf != 0;
+                        inChain = 0;
+                    }
+                }
+            }
+        }
+    }
+    else if (warp >= 4)
+    {
+        const int rw = warp - 4, quad = rw & 3, half = rw >> 2;
+        if (rw < resultWarps)
+        {
+            const int cols = bn > 128 ? 128 : bn;
+            const unsigned mine = tm + ((unsigned) (quad * 32) << 16) + half * 128;
+            const int m = quad * 32 + lane;
+            Chains chain;
+            for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
+            {
+                const long long m0 = (long long) (tile % a.tilesM) * 128, n0 = (long long) (tile / a.tilesM) * bn;
+                float acc[128];
+#pragma unroll
+                for (int j = 0; j < 128; ++j)
+                    acc[j] = 0.0f;
+                const float bias = a.bias && a.splits == 1 && m0 + m < a.O ? a.bias[m0 + m] : 0.0f;
+                for (int i = 0; i < count; i += CHAIN_STEPS, chain.next(bufs))
+                    take_chain(&bars, chain.buf, chain.par, mine + chain.buf * 128, cols, i == 0, acc);
+                if (a.splits > 1)
+                    put_partial<false>(reinterpret_cast<float*>(stage0), bn, m, half * 128, cols, acc);
+                else
+                    write_columns((T*) a.y, a.ld, m0 + m, a.O, n0 + half * 128, a.T, cols, acc, bias, lane ^ 1, a.pairs && m0 + 128 <= a.O);
+            }
+        }
+    }
+    __syncwarp();
+    if (a.splits > 1) // one tile per cluster
+        reduce_cluster<false, T>(reinterpret_cast<float*>(stage0), a.splits, rank, bn, (T*) a.y, a.ld, (long long) (blockIdx.x % a.tilesM) * 128, a.O,
+                                 (long long) (blockIdx.x / a.tilesM) * bn, a.T, a.bias, false);
     tc_fence_before();
     __syncthreads();
     if (warp == 2)
@@ -301,40 +495,61 @@ struct GradArgs
     long long I;        // rows of the packed matrix: lanes of the tile
     long long C;        // columns of the packed matrix: the contraction
     long long N;        // the other dimension
-    int bn, stages, splits, vec, add;
+    int bn, stages, splits, tilesM, tiles;
+    int vec;            // dy can be read 16 bytes a time
+    int wide;           // out: rows can be written 16 bytes a time, columns in pairs of rows
+    int add;
 };
 
 constexpr int GK = 64; // contraction values per stage
+
+// Threads, in groups of four warps: copy / product / allocating / spare; expanding; result; with a dense operand that the copy engine
+// cannot take, one group less of the second and third kind and four of loaders.  The threads are launched with as many registers
+// each as the SM has for all of them, and redistribute them.
+// Tensor memory: two accumulators of 192 columns and four expanded steps of 32, or, tiles being 128 wide with loaders, two of 128
+// and eight.  A 192-wide tile reads 6 % more per product than one of 256, which would leave room for one accumulator.
+constexpr int GRAD_WIDEST = 192, GRAD_WIDEST_DENSE = 128;
+template <bool DENSE>
+struct GradGroups
+{
+    static constexpr int expand = DENSE ? 1 : 3, result = DENSE ? 1 : 2, load = DENSE ? 4 : 0;
+    static constexpr int firstExpand = 4, firstResult = firstExpand + 4 * expand, firstLoad = firstResult + 4 * result;
+    static constexpr int threads = 128 * (1 + expand + result + load);
+    static constexpr int regsLaunch = DENSE ? 72 : 80; // 65536 / threads, a multiple of 8
+    static constexpr int regsMisc = DENSE ? 40 : 56, regsExpand = 56, regsResult = DENSE ? 152 : 128, regsLoad = 64;
+    static_assert(regsLaunch * threads <= 65536 && 128 * (regsMisc + regsExpand * expand + regsResult * result + regsLoad * load) <= regsLaunch * threads, "registers");
+};
 
 __host__ __device__ inline int grad_codes_bytes(int format)
 {
     return GK * (format == QAGG_MXFP4 ? 64 : 128);
 }
 
-// Two values of this lane, k and k + 1, as bf16: codes b0, b1 (fp4: the byte that holds the value, `nib` the shift to it) times the
-// scale pair.  int8: 0x43 over a code byte is the bf16 number 128 + (its low seven bits) with bit 7 moved aside; q = low - (bit 7),
-// so q = (128 + low) - (128 or 256), and 256 is 0x4380.  fp4: exponent and mantissa bits set where bf16 has them give the value
-// times 2^-126, subnormal included.
-template <int FMT>
-__device__ __forceinline__ unsigned expand2(unsigned b0, unsigned b1, unsigned nib, unsigned scale)
+// Codes to bf16.  v: four codes of one row (int8), or four bytes with one code of an even and one of an odd row each (fp4), from
+// contraction values k..k+3; pair 0 is (k, k + 1), pair 1 (k + 2, k + 3).
+// int8: 0x43 over a code byte is the bf16 number 128 + (its low seven bits) with bit 7 moved aside; q = low - (bit 7), so
+// q = (128 + low) - (128 or 256), and 256 is 0x4380.  fp4: the element's exponent and mantissa bits, set where bf16 has them, give
+// its value times 2^-126, subnormal included.  All products are exact.
+__device__ __forceinline__ unsigned bf16x2_mul(unsigned a, unsigned b)
 {
-    unsigned v = b0 + (b1 << 16), r;
-    if constexpr (FMT == QAGG_MXINT8)
-    {
-        const unsigned mag = (v & 0x007f007fu) | 0x43004300u, sub = (v & 0x00800080u) | 0x43004300u;
-        const __nv_bfloat162 q = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&mag), *reinterpret_cast<const __nv_bfloat162*>(&sub));
-        const __nv_bfloat162 e = __hmul2(q, *reinterpret_cast<const __nv_bfloat162*>(&scale));
-        r = *reinterpret_cast<const unsigned*>(&e);
-    }
-    else
-    {
-        v >>= nib;
-        const unsigned t = ((v << 6) & 0x01c001c0u) | ((v << 12) & 0x80008000u), up = 0x7e807e80u; // 2^126
-        const __nv_bfloat162 q = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&t), *reinterpret_cast<const __nv_bfloat162*>(&up));
-        const __nv_bfloat162 e = __hmul2(q, *reinterpret_cast<const __nv_bfloat162*>(&scale));
-        r = *reinterpret_cast<const unsigned*>(&e);
-    }
-    return r;
+    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const unsigned*>(&r);
+}
+__device__ __forceinline__ unsigned bf16x2_sub(unsigned a, unsigned b)
+{
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const unsigned*>(&r);
+}
+__device__ __forceinline__ unsigned expand_int8(unsigned v, int pair, unsigned scale)
+{
+    const unsigned x = __byte_perm(v, 0x43434343u, pair ? 0x4342 : 0x4140);
+    return bf16x2_mul(bf16x2_sub(x & 0xff7fff7fu, x & 0xff80ff80u), scale);
+}
+__device__ __forceinline__ unsigned expand_fp4(unsigned v, int pair, bool odd, unsigned scale)
+{
+    const unsigned x = __byte_perm(v, 0, pair ? 0x4342 : 0x4140);
+    const unsigned t = odd ? ((x << 2) & 0x01c001c0u) | ((x << 8) & 0x80008000u) : ((x << 6) & 0x01c001c0u) | ((x << 12) & 0x80008000u);
+    return bf16x2_mul(bf16x2_mul(t, 0x7e807e80u), scale); // 2^126
 }
 // multiplier of a block as bf16 bits: 2^X (fp4), 2^X / 64 (int8; subnormal below byte 7)
 template <int FMT>
@@ -347,210 +562,412 @@ __device__ __forceinline__ unsigned scale_bf16(unsigned byte)
     return byte ? byte << 7 : 0x40u;
 }
 
-// A dense value as a sum of bf16 planes, exactly: the top eight significant bits by truncation, the next eight, the rest (fp16 has
-// eleven: two planes; fp32 twenty-four: three).  Infinities and NaN stay in the first plane.
-template <class T, int NP>
-__device__ __forceinline__ void split_planes(T x, unsigned short (&p)[NP])
+// Eight dense values as sums of bf16 planes, exactly: the top eight significant bits by truncation, the next eight, the rest (fp16 has
+// eleven: two planes; fp32 twenty-four: three).  Infinities and NaN stay in the first plane, which the second form sees to.
+template <class T, int NP, bool SPECIAL>
+__device__ __forceinline__ void split8(const Raw8<T>& raw, unsigned (&w)[NP][4])
 {
-    if constexpr (NP == 1)
-        p[0] = __bfloat16_as_ushort((__nv_bfloat16) x);
-    else
-    {
-        float v = (float) x;
-        const bool finite = (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u;
-        if (!finite)
-        {
-            p[0] = v != v ? 0x7fff : (unsigned short) (__float_as_uint(v) >> 16);
+    const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-            for (int k = 1; k < NP; ++k)
-                p[k] = 0;
-            return;
-        }
+    for (int i = 0; i < 4; ++i)
+    {
+        float v[2] = {(float) e[2 * i], (float) e[2 * i + 1]};
 #pragma unroll
         for (int k = 0; k < NP; ++k)
         {
-            const unsigned top = __float_as_uint(v) & 0xffff0000u;
-            p[k] = (unsigned short) (top >> 16);
-            v -= __uint_as_float(top);
+            unsigned top[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+            {
+                const unsigned bits = __float_as_uint(v[h]);
+                const bool special = SPECIAL && (bits & 0x7f800000u) == 0x7f800000u;
+                top[h] = special && v[h] != v[h] ? 0x7fff0000u : bits;
+                if (k + 1 < NP)
+                    v[h] = special ? 0.0f : v[h] - __uint_as_float(bits & 0xffff0000u);
+            }
+            w[k][i] = __byte_perm(top[0], top[1], 0x7632);
         }
     }
+}
+template <class T>
+__device__ __forceinline__ bool any_special(const Raw8<T>& raw)
+{
+    const T* e = reinterpret_cast<const T*>(&raw);
+    float zero = 0.0f; // stays 0 unless a value is infinite or NaN
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        zero = __fmaf_rn((float) e[i], 0.0f, zero);
+    return zero != 0.0f;
 }
 
 // WEIGHT: dw, lanes = i, columns = o, contraction over the tokens; the dense operand is MN-major (o runs fastest).
 // otherwise: dx, lanes = i, columns = t, contraction over o; the dense operand is K-major.
-// DENSE 0: dy is bf16 and the copy engine can take it.  DENSE 1..3: that many bf16 planes, made by eight loader warps from T.
+// DENSE 0: dy is bf16 and the copy engine can take it.  DENSE 1..3: that many bf16 planes, made by loader warps from TD.
 template <bool WEIGHT, int FMT, int DENSE, class TD, class TO>
-__global__ void __launch_bounds__(DENSE ? GT_DENSE : GT, 1) k_mx_grad(const __grid_constant__ CUtensorMap mapCodes, const __grid_constant__ CUtensorMap mapDy, const GradArgs a)
+__global__ void __launch_bounds__(GradGroups<(DENSE > 0)>::threads, 1) k_mx_grad(const __grid_constant__ CUtensorMap mapCodes, const __grid_constant__ CUtensorMap mapDy, const GradArgs a)
 {
+    using G = GradGroups<(DENSE > 0)>;
     constexpr int NP = DENSE ? DENSE : 1;
+    constexpr int CHAIN_STEPS = (sizeof(TO) == 4 ? CHAIN : CHAIN_16BIT) / 4 / NP;
+    constexpr int WIDEST = DENSE ? GRAD_WIDEST_DENSE : GRAD_WIDEST;
+    constexpr unsigned SIDE = 2 * WIDEST;
+    constexpr int SLOTS = (TMEM_COLS - SIDE) / 32; // expanded steps in tensor memory
     extern __shared__ unsigned char dyn[];
     __shared__ GemmBars bars;
-    __shared__ unsigned scalePairs[8][2][16];
+    __shared__ __align__(16) unsigned short scaleRows[4 * G::expand][GK]; // per expanding warp: its block's multipliers for one step
     unsigned char* stage0 = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t) 1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int bn = a.bn, S = a.stages;
     const int denseBytes = bn * 128 * NP;
     const int stageBytes = denseBytes + grad_codes_bytes(FMT);
-    const long long m0 = (long long) blockIdx.x * 128, n0 = (long long) blockIdx.y * bn;
     const int steps = (int) ((a.C + GK - 1) / GK);
     const int rank = a.splits > 1 ? (int) cluster_rank() : 0;
     int first, count;
     split_range(steps, rank, a.splits, first, count);
+    constexpr int resultWarps = 4 * G::result;
+    auto tile_m0 = [&](int tile) { return (long long) (tile % a.tilesM) * 128; };
+    auto tile_n0 = [&](int tile) { return (long long) (tile / a.tilesM) * bn; };
 
-    gemm_setup(&bars, S, 8, 8);
+    auto copy_step = [&](int tile, int i, int s) {
+        const int m0 = (int) tile_m0(tile), n0 = (int) tile_n0(tile);
+        const unsigned at = smem_addr(stage0) + s * stageBytes;
+        const int k0 = (first + i) * GK;
+        mbar_arrive_expect_tx(&bars.full[s], grad_codes_bytes(FMT) + (DENSE ? 0 : denseBytes));
+        tma_load_2d(at + denseBytes, &mapCodes, FMT == QAGG_MXFP4 ? m0 / 2 : m0, k0, &bars.full[s]);
+        if constexpr (DENSE == 0)
+        {
+            if constexpr (WEIGHT)
+                for (int n = 0; n < bn; n += 64)
+                    tma_load_2d(at + n * 128, &mapDy, n0 + n, k0, &bars.full[s]);
+            else
+                tma_load_2d(at, &mapDy, k0, n0, &bars.full[s]);
+        }
+    };
+    int early = 0; // steps of the first tile whose copies start before the CTA has met
+    if (warp == 0)
+    {
+        if (elect_one())
+        {
+            init_barriers(&bars, S, 4, 4 * G::load, resultWarps);
+            for (; early < count && early < S; ++early)
+                copy_step(blockIdx.x, early, early);
+        }
+        early = count < S ? count : S;
+        __syncwarp();
+    }
+    if (warp == 2)
+        tmem_alloc(&bars.tmem, TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
     const unsigned tm = bars.tmem;
-    const unsigned tmA = tm + 256; // 32 columns a stage
-    if (warp == 0 && lane == 0)
+    const unsigned tmA = tm + SIDE;
+
+    if (warp < 4)
     {
-        for (int i = 0; i < count; ++i)
+        registers_down<G::regsMisc>();
+        if (warp == 0 && elect_one())
         {
-            const int s = i % S;
-            if (i >= S)
-                tc_wait(&bars.empty[s], ((i / S) & 1) ^ 1, &bars.broken, &g_mxStatus);
-            if (*reinterpret_cast<volatile unsigned*>(&bars.broken))
-            {
-                drain_copies(&bars, i, S);
-                break;
-            }
-            const unsigned at = smem_addr(stage0 + (size_t) s * stageBytes);
-            const int k0 = (first + i) * GK;
-            mbar_arrive_expect_tx(&bars.full[s], grad_codes_bytes(FMT) + (DENSE ? 0 : denseBytes));
-            tma_load_2d(at + denseBytes, &mapCodes, (int) (FMT == QAGG_MXFP4 ? m0 / 2 : m0), k0, &bars.full[s]);
-            if constexpr (DENSE == 0)
-            {
-                if constexpr (WEIGHT)
-                    for (int n = 0; n < bn; n += 64)
-                        tma_load_2d(at + n * 128, &mapDy, (int) n0 + n, k0, &bars.full[s]);
-                else
-                    tma_load_2d(at, &mapDy, k0, (int) n0, &bars.full[s]);
-            }
-        }
-    }
-    else if (warp == 1 && lane == 0)
-    {
-        const unsigned idesc = idesc_bf16(bn, WEIGHT);
-        for (int i = 0; i < count; ++i)
-        {
-            const int s = i % S;
-            const unsigned par = (i / S) & 1;
-            tc_wait(&bars.full[s], par, &bars.broken, &g_mxStatus);
-            if constexpr (DENSE > 0)
-                tc_wait(&bars.dense[s], par, &bars.broken, &g_mxStatus);
-            tc_wait(&bars.conv[s], par, &bars.broken, &g_mxStatus);
-            tc_fence_after();
-            const unsigned at = smem_addr(stage0 + (size_t) s * stageBytes);
-            // smallest plane first: its products are added while the sum of this step is small
-#pragma unroll
-            for (int p = NP - 1; p >= 0; --p)
-#pragma unroll
-                for (int j = 0; j < GK / 16; ++j)
+            Ring ring;
+            for (int i = 0; i < early; ++i)
+                ring.next(S);
+            long long issued = early;
+            for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
+                for (int i = tile == (int) blockIdx.x ? early : 0; i < count; ++i, ++issued)
                 {
-                    const unsigned b = at + p * bn * 128;
-                    const unsigned long long desc = WEIGHT ? smem_desc(b + j * 2048, 8192, 1024, SWIZZLE_128B) : smem_desc(b + j * 32, 16, 1024, SWIZZLE_128B);
-                    mma_bf16_ts(tm, tmA + s * 32 + j * 8, desc, idesc, i > 0 || j > 0 || p < NP - 1);
+                    if (issued >= S)
+                        tc_wait(&bars.empty[ring.s], ring.par ^ 1, &bars.broken, &g_mxStatus);
+                    if (*reinterpret_cast<volatile unsigned*>(&bars.broken))
+                    {
+                        drain_copies(&bars, issued, S);
+                        tile = a.tiles;
+                        break;
+                    }
+                    copy_step(tile, i, ring.s);
+                    ring.next(S);
                 }
-            tc_commit(&bars.empty[s]);
         }
-        tc_commit(&bars.done);
+        else if (warp == 1 && elect_one())
+        {
+            Ring ring;
+            Chains chain;
+            bool fresh = true; // accumulators that no chain has used
+            int slot = 0;
+            const unsigned idesc = idesc_bf16(bn, WEIGHT);
+            const unsigned long long d0 = WEIGHT ? smem_desc(smem_addr(stage0), 8192, 1024, SWIZZLE_128B) : smem_desc(smem_addr(stage0), 16, 1024, SWIZZLE_128B);
+            constexpr unsigned KSTEP = (WEIGHT ? 2048 : 32) >> 4;
+            for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
+            {
+                int inChain = 0;
+                for (int i = 0; i < count; ++i)
+                {
+                    if (inChain == 0 && !fresh)
+                        tc_wait(&bars.taken[chain.buf], chain.par ^ 1, &bars.broken, &g_mxStatus);
+                    // the expanding warps saw the copies land before they arrived
+                    if constexpr (DENSE > 0)
+                        tc_wait(&bars.dense[ring.s], ring.par, &bars.broken, &g_mxStatus);
+                    tc_wait(&bars.conv[ring.s], ring.par, &bars.broken, &g_mxStatus);
+                    tc_fence_after();
+                    const unsigned long long d = d0 + ((unsigned) (ring.s * stageBytes) >> 4);
+                    const unsigned ta = tmA + slot * 32, acc = tm + chain.buf * WIDEST;
+                    slot = (slot + 1) % SLOTS;
+#pragma unroll
+                    for (int p = 0; p < NP; ++p)
+#pragma unroll
+                        for (int j = 0; j < GK / 16; ++j)
+                            mma_bf16_ts(acc, ta + j * 8, d + p * (bn * 128 >> 4) + j * KSTEP, idesc, inChain > 0 || p + j > 0);
+                    tc_commit(&bars.empty[ring.s]);
+                    ring.next(S);
+                    if (++inChain == CHAIN_STEPS || i + 1 == count)
+                    {
+                        tc_commit(&bars.ready[chain.buf]);
+                        chain.next(2);
+                        fresh = fresh && chain.buf != 0;
+                        inChain = 0;
+                    }
+                }
+            }
+        }
     }
-    else if (warp >= 4 && warp < 12)
+    else if (warp < G::firstResult)
     {
-        // expand: lanes 32 * quad .. are one block of the packed matrix; this warp takes 32 of the stage's 64 contraction values
-        const int quad = warp & 3, half = (warp - 4) >> 2;
-        const long long tilesM = mx_scale_tiles(a.I);
-        const unsigned nib = FMT == QAGG_MXFP4 ? (lane & 1) * 4 : 0;
-        const unsigned char* mine = a.scales + (m0 / 128) * 512 + lane * 16 + quad;
-        auto fetch = [&](int i) -> unsigned {
-            const long long k = (long long) (first + i) * GK + half * 32; // the scale tiles cover whole groups of 128 columns
-            return mine[k / 128 * tilesM * 512 + (k % 128) / 32 * 4];
+        registers_down<G::regsExpand>();
+        // Expand: lanes 32 * quad .. of the tile are one block of the packed matrix, so a warp has one scale per contraction value.
+        // The codes lie [contraction value][row]; ldmatrix transposes 16 x 16 bytes of them into the order in which a 16 x 256-bit
+        // store to tensor memory takes pairs of contraction values.  With fp4 that puts row 16 h + 2 b + o of the block on lane
+        // 16 h + 8 o + b; the result warps know.  Several groups of warps take the steps in turn.
+        const int quad = warp & 3, group = (warp - G::firstExpand) >> 2;
+        const long long tileRow = mx_scale_tiles(a.I) * 512;
+        unsigned short* mult = scaleRows[warp - G::firstExpand];
+        // rows of the code tile are 128 (fp4: 64) bytes, their 16-byte pieces swizzled by the copy
+        constexpr int ROW = FMT == QAGG_MXFP4 ? 64 : 128;
+        unsigned rowAt[2]; // this lane's row address for ldmatrix, for each 16 rows of the block (fp4: one piece holds all 32)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+        {
+            const int piece = FMT == QAGG_MXFP4 ? quad : quad * 2 + h;
+            rowAt[h] = smem_addr(stage0) + denseBytes + lane * ROW + ((FMT == QAGG_MXFP4 ? piece ^ ((lane >> 1) & 3) : piece ^ (lane & 7)) << 4);
+        }
+        // Slot n % SLOTS of tensor memory is free when the products of step n - SLOTS are done.  With no more stages than slots the
+        // copies of this step had to wait for them already.  With more, their stage has been handed back, and cannot be handed back
+        // once more (which would make the parity ambiguous) before this warp has done its part of step n - SLOTS + stages > n.
+        int n = 0, stage = 0, oldStage = SLOTS < S ? S - SLOTS : 0, slot = 0; // n: step, over all tiles; oldStage: that of step n - SLOTS
+        unsigned par = 0, oldPar = 1;                                      // parities of their rounds
+        auto advance = [&](int k) { // k <= G::expand <= S, SLOTS
+            n += k;
+            slot = (slot + k) % SLOTS;
+            if ((stage += k) >= S)
+            {
+                stage -= S;
+                par ^= 1;
+            }
+            if ((oldStage += k) >= S)
+            {
+                oldStage -= S;
+                oldPar ^= 1;
+            }
         };
-        unsigned byte = count > 0 ? fetch(0) : 0;
-        for (int i = 0; i < count; ++i)
+        for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
         {
-            const int s = i % S;
-            unsigned* pairs = scalePairs[warp - 4][i & 1];
-            const unsigned mineScale = scale_bf16<FMT>(byte);
-            const unsigned next = __shfl_down_sync(0xffffffffu, mineScale, 1);
-            if ((lane & 1) == 0)
-                pairs[lane / 2] = mineScale | (next << 16);
-            if (i + 1 < count)
-                byte = fetch(i + 1);
-            __syncwarp();
-            tc_wait(&bars.full[s], (i / S) & 1, &bars.broken, &g_mxStatus);
-            __syncwarp();
-            const unsigned char* codes = stage0 + (size_t) s * stageBytes + denseBytes +
-                                         (FMT == QAGG_MXFP4 ? half * 32 * 64 + quad * 16 + lane / 2 : half * 32 * 128 + quad * 32 + lane);
-            constexpr int ROW = FMT == QAGG_MXFP4 ? 64 : 128;
-            unsigned r[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-                r[j] = expand2<FMT>(codes[(2 * j) * ROW], codes[(2 * j + 1) * ROW], nib, pairs[j]);
-            tc_fence_after(); // the stage's previous products, whose end the copy warp saw, have read this part of tensor memory
-            tmem_store16(tmA + ((unsigned) (quad * 32) << 16) + s * 32 + half * 16, r);
-            tmem_store_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0)
-                mbar_arrive(&bars.conv[s]);
-        }
-    }
-    else if (DENSE > 0 && warp >= 12)
-    {
-        // bring the dense operand: rows of 64 contiguous values (128 bytes a plane), eight values a thread and turn
-        const TD* dy = (const TD*) a.dy;
-        const int t = threadIdx.x - GT;
-        for (int i = 0; i < count; ++i)
-        {
-            const int s = i % S;
-            if (i >= S)
-                tc_wait(&bars.empty[s], ((i / S) & 1) ^ 1, &bars.broken, &g_mxStatus);
-            unsigned char* at = stage0 + (size_t) s * stageBytes;
-            const long long k0 = (long long) (first + i) * GK;
-            for (int u = t; u < bn * 8; u += 256)
+            const unsigned char* mine = a.scales + tile_m0(tile) / 128 * 512 + lane * 16 + quad;
+            auto fetch = [&](int i, unsigned& b0, unsigned& b1) { // the scale tiles cover whole groups of 128 columns
+                const unsigned k = (unsigned) (first + i) * GK;
+                const unsigned char* p = mine + (long long) (k / 128) * tileRow + (k & 64) / 8;
+                b0 = p[0];
+                b1 = p[4];
+            };
+            unsigned b0 = 0, b1 = 0;
+            int i = 0;
+            for (; i < count && n % G::expand != group; ++i) // steps of the other groups
+                advance(1);
+            if (i < count)
+                fetch(i, b0, b1);
+            for (; i < count; i += G::expand)
             {
-                // row r of piece `atom` in the stage; its place in dy
-                const int c = u & 7, r = WEIGHT ? (u >> 3) & 63 : u >> 3, atom = WEIGHT ? u >> 9 : 0;
-                const long long line = WEIGHT ? k0 + r : n0 + r;               // token
-                const long long col = (WEIGHT ? n0 + atom * 64 : k0) + c * 8;   // output
-                const long long lines = WEIGHT ? a.C : a.N, cols = WEIGHT ? a.N : a.C;
-                TD v[8];
-                const TD* src = dy + line * a.ldDy + col;
-                if (line < lines && col + 8 <= cols && a.vec)
+                __syncwarp();
+                mult[lane] = (unsigned short) scale_bf16<FMT>(b0);
+                mult[lane + 32] = (unsigned short) scale_bf16<FMT>(b1);
+                if (i + G::expand < count)
+                    fetch(i + G::expand, b0, b1);
+                __syncwarp();
+                tc_wait(&bars.full[stage], par, &bars.broken, &g_mxStatus);
+                __syncwarp();
+                if (S > SLOTS && n >= SLOTS)
                 {
-                    uint4* q = reinterpret_cast<uint4*>(v);
-                    q[0] = *reinterpret_cast<const uint4*>(src);
-                    if constexpr (sizeof(TD) == 4)
-                        q[1] = *(reinterpret_cast<const uint4*>(src) + 1);
+                    tc_wait(&bars.empty[oldStage], oldPar, &bars.broken, &g_mxStatus);
+                    __syncwarp();
+                }
+                tc_fence_after();
+                const unsigned off = stage * stageBytes;
+                const unsigned to = tmA + ((unsigned) (quad * 32) << 16) + slot * 32;
+                uint2 sc[4]; // multipliers of contraction values 16 g + 4 (lane % 4) .. + 3
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    sc[g] = *reinterpret_cast<const uint2*>(mult + 16 * g + 4 * (lane & 3));
+                // piece g of a block half is 16 contraction values: two registers
+                if constexpr (FMT == QAGG_MXINT8)
+                {
+                    unsigned c[2][8];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                    {
+                        ldmatrix_trans_b8(rowAt[h] + off, reinterpret_cast<unsigned(&)[4]>(c[h][0]));
+                        ldmatrix_trans_b8(rowAt[h] + off + 32 * ROW, reinterpret_cast<unsigned(&)[4]>(c[h][4]));
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                    {
+                        unsigned r[16];
+#pragma unroll
+                        for (int g = 0; g < 4; ++g)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                            {
+                                r[4 * g + 2 * e] = expand_int8(c[h][2 * g + e], 0, sc[g].x);
+                                r[4 * g + 2 * e + 1] = expand_int8(c[h][2 * g + e], 1, sc[g].y);
+                            }
+                        tmem_store_16x256b(to + ((unsigned) (h * 16) << 16), r);
+                    }
                 }
                 else
                 {
+                    unsigned c[8], r[16];
+                    ldmatrix_trans_b8(rowAt[0] + off, reinterpret_cast<unsigned(&)[4]>(c[0]));
+                    ldmatrix_trans_b8(rowAt[0] + off + 32 * ROW, reinterpret_cast<unsigned(&)[4]>(c[4]));
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        v[e] = line < lines && col + e < cols ? src[e] : (TD) 0.0f;
+                    for (int h = 0; h < 2; ++h)
+                    {
+#pragma unroll
+                        for (int g = 0; g < 4; ++g)
+#pragma unroll
+                            for (int o = 0; o < 2; ++o)
+                            {
+                                r[4 * g + 2 * o] = expand_fp4(c[2 * g + h], 0, o, sc[g].x);
+                                r[4 * g + 2 * o + 1] = expand_fp4(c[2 * g + h], 1, o, sc[g].y);
+                            }
+                        tmem_store_16x256b(to + ((unsigned) (h * 16) << 16), r);
+                    }
                 }
-                unsigned short pl[8][NP];
+                tmem_store_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(&bars.conv[stage]);
+                advance(min(G::expand, count - i));
+            }
+        }
+    }
+    else if (warp < G::firstLoad)
+    {
+        registers_up<G::regsResult>();
+        const int rw = warp - G::firstResult, quad = rw & 3, half = rw >> 2;
+        {
+            const int cols = bn / G::result;
+            const unsigned mine = tm + ((unsigned) (quad * 32) << 16) + half * cols;
+            const int m = quad * 32 + (FMT == QAGG_MXFP4 ? (lane & 16) + 2 * (lane & 7) + ((lane >> 3) & 1) : lane);
+            Chains chain;
+            for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
+            {
+                const long long m0 = tile_m0(tile), n0 = tile_n0(tile);
+                constexpr int ACC = WIDEST / G::result;
+                float acc[ACC];
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    split_planes<TD, NP>(v[e], pl[e]);
+                for (int j = 0; j < ACC; ++j)
+                    acc[j] = 0.0f;
+                for (int i = 0; i < count; i += CHAIN_STEPS, chain.next(2))
+                    take_chain(&bars, chain.buf, chain.par, mine + chain.buf * WIDEST, cols, i == 0, acc);
+                if (a.splits > 1)
+                    put_partial<WEIGHT>(reinterpret_cast<float*>(stage0), bn, m, half * cols, cols, acc);
+                else if constexpr (WEIGHT)
+                    write_row((float*) a.out, a.ld, m0 + m, a.I, n0 + half * cols, a.N, cols, acc, a.add != 0, a.wide != 0);
+                else
+                    write_columns((TO*) a.out, a.ld, m0 + m, a.I, n0 + half * cols, a.N, cols, acc, 0.0f, lane ^ (FMT == QAGG_MXFP4 ? 8 : 1), a.wide && m0 + 128 <= a.I);
+            }
+        }
+    }
+    else
+    {
+        // Bring the dense operand: rows of 64 contiguous values (128 bytes a plane), eight values a thread and turn.  Two steps' values
+        // are on their way (behind the fence, which would wait for them) while an earlier one is split and stored.
+        registers_down<G::regsLoad>();
+        const TD* dy = (const TD*) a.dy;
+        const int t = threadIdx.x - G::firstLoad * 32;
+        constexpr int UNITS = 2; // bn <= 128: at most 1024 pieces for 512 threads
+        struct Step
+        {
+            Raw8<TD> raw[UNITS];
+        };
+        int nextTile = blockIdx.x, nextStep = 0;
+        auto fetch = [&](Step& st) { // the next step that this CTA has
+            if (nextTile >= a.tiles || count == 0)
+                return;
+            const long long n0 = tile_n0(nextTile), k0 = (long long) (first + nextStep) * GK;
+#pragma unroll
+            for (int q = 0; q < UNITS; ++q)
+            {
+                const int u = t + q * 512;
+                const int c = u & 7, r = WEIGHT ? (u >> 3) & 63 : u >> 3, atom = WEIGHT ? u >> 9 : 0;
+                const long long line = WEIGHT ? k0 + r : n0 + r;              // token
+                const long long col = (WEIGHT ? n0 + atom * 64 : k0) + c * 8; // output
+                const long long left = (WEIGHT ? a.N : a.C) - col;
+                st.raw[q] = load8(dy + line * a.ldDy + col, u < bn * 8 && line < (WEIGHT ? a.C : a.N) ? (left < 0 ? 0 : left < 8 ? (int) left : 8) : 0, a.vec);
+            }
+            if (++nextStep == count)
+            {
+                nextStep = 0;
+                nextTile += gridDim.x;
+            }
+        };
+        Ring ring;
+        long long done = 0;
+        auto put_step = [&](Step& st) {
+            if (done >= S)
+                tc_wait(&bars.empty[ring.s], ring.par ^ 1, &bars.broken, &g_mxStatus);
+            ++done;
+            unsigned char* at = stage0 + ring.s * stageBytes;
+#pragma unroll
+            for (int q = 0; q < UNITS; ++q)
+            {
+                const int u = t + q * 512;
+                const int c = u & 7, r = WEIGHT ? (u >> 3) & 63 : u >> 3, atom = WEIGHT ? u >> 9 : 0;
                 unsigned char* dst = at + atom * 8192 + r * 128 + ((c ^ (r & 7)) << 4);
+                unsigned w[NP][4];
+                if (NP == 1)
+                    *reinterpret_cast<uint4*>(w[0]) = st.raw[q].a;
+                else if (any_special(st.raw[q]))
+                    split8<TD, NP, true>(st.raw[q], w);
+                else
+                    split8<TD, NP, false>(st.raw[q], w);
 #pragma unroll
                 for (int p = 0; p < NP; ++p)
-                    *reinterpret_cast<uint4*>(dst + p * bn * 128) =
-                        make_uint4(pl[0][p] | (unsigned) pl[1][p] << 16, pl[2][p] | (unsigned) pl[3][p] << 16, pl[4][p] | (unsigned) pl[5][p] << 16,
-                                   pl[6][p] | (unsigned) pl[7][p] << 16);
+                    if (u < bn * 8)
+                        *reinterpret_cast<uint4*>(dst + p * bn * 128) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
             }
             fence_async_shared();
             __syncwarp();
             if (lane == 0)
-                mbar_arrive(&bars.dense[s]);
+                mbar_arrive(&bars.dense[ring.s]);
+            ring.next(S);
+        };
+        Step even, odd;
+        fetch(even);
+        fetch(odd);
+        const long long mySteps = (int) blockIdx.x < a.tiles ? (long long) ((a.tiles - 1 - (int) blockIdx.x) / (int) gridDim.x + 1) * count : 0;
+        for (long long n = 0; n < mySteps; n += 2)
+        {
+            put_step(even);
+            fetch(even);
+            if (n + 1 < mySteps)
+            {
+                put_step(odd);
+                fetch(odd);
+            }
         }
     }
     __syncwarp();
-    tc_wait(&bars.done, 0, &bars.broken, &g_mxStatus);
-    __syncwarp();
-    tc_fence_after();
-    const int resultWarp = warp < 12 ? warp - 4 : -1;
-    write_tile<WEIGHT, TO>(tm, count == 0, bn, resultWarp, reinterpret_cast<float*>(stage0), a.splits, rank, (TO*) a.out, a.ld, m0, a.I, n0, a.N, nullptr, a.add != 0);
+    if (a.splits > 1) // one tile per cluster
+        reduce_cluster<WEIGHT, TO>(reinterpret_cast<float*>(stage0), a.splits, rank, bn, (TO*) a.out, a.ld, tile_m0(blockIdx.x), a.I, tile_n0(blockIdx.x), a.N, nullptr,
+                                   a.add != 0);
     tc_fence_before();
     __syncthreads();
     if (warp == 2)
@@ -559,27 +976,31 @@ __global__ void __launch_bounds__(DENSE ? GT_DENSE : GT, 1) k_mx_grad(const __gr
 
 // ---- launches -----------------------------------------------------------------------------------------------------------------
 
-// Tile width and split of the contraction.  Costs in units of a 256-wide step: a CTA runs steps / splits of them, then its result.
+// Tile width and split of the contraction, by a count of cycles: a CTA runs waves * steps / splits steps, each as long as its products
+// (2 * bn * planes: 8192 bf16 or 32768 fp4 multiply-adds a cycle) or its copies (64 bytes a cycle from L2) take, whichever is more;
+// then the last tile's result goes out.
 struct Shape
 {
     int bn, splits;
 };
-static Shape choose_shape(long long tilesM, long long N, int steps, int sms, int widest, int narrowest)
+static Shape choose_shape(long long tilesM, long long N, int steps, int sms, const int* widths, int nWidths, int planes, int fixedBytes, int columnBytes)
 {
-    Shape best = {widest, 1};
+    Shape best = {widths[0], 1};
     double bestCost = 1e300;
-    for (int bn = widest; bn >= narrowest; bn /= 2)
+    for (int i = 0; i < nWidths; ++i)
     {
-        if (bn < widest && bn < 128 && N > bn)
+        const int bn = widths[i];
+        if (i > 0 && bn < 128 && N > bn)
             break; // several narrow tiles would read the other operand once each
         const long long tiles = tilesM * ((N + bn - 1) / bn);
+        const double step = 50.0 + std::max(2.0 * bn * planes, (fixedBytes + (double) bn * columnBytes) / 64.0);
         for (int s = 1; s <= 8; s *= 2)
         {
             if (s > 1 && s > steps)
                 break;
             const long long waves = (tiles * s + sms - 1) / sms;
-            const double step = std::max(bn, 96) / 256.0;
-            const double cost = waves * (step * ((steps + s - 1) / s) + 4.0 + 6.0 * bn / 256.0 + (s > 1 ? 2.0 : 0.0));
+            // split: every wave starts anew and ends with an exchange; otherwise tiles follow one another without a gap
+            const double cost = step * waves * ((steps + s - 1) / s) + (s > 1 ? waves * (5000.0 + 4.0 * bn) : 3000.0 + 4.0 * bn);
             if (cost < bestCost)
             {
                 bestCost = cost;
@@ -621,9 +1042,10 @@ static cudaError_t launch_cluster(K kernel, dim3 grid, int threads, int smem, in
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-static bool codes_map(CUtensorMap* m, const void* codes, long long M, long long N, int format, int boxBytes, int boxCols, bool swizzle)
+// boxes of boxBytes x boxCols codes, the 16-byte pieces of a row swizzled within it
+static bool codes_map(CUtensorMap* m, const void* codes, long long M, long long N, int format, int boxBytes, int boxCols)
 {
-    return encode_map_tiled(m, 1, codes, mx_pitch(M, format), N, mx_pitch(M, format), boxBytes, boxCols, swizzle);
+    return encode_map_tiled(m, 1, codes, mx_pitch(M, format), N, mx_pitch(M, format), boxBytes, boxCols, boxBytes);
 }
 
 template <bool WEIGHT, int FMT, int DENSE, class TD, class TO>
@@ -632,9 +1054,9 @@ static cudaError_t launch_grad(cudaStream_t st, const CUtensorMap& mc, const CUt
     constexpr int NP = DENSE ? DENSE : 1;
     const int stageBytes = a.bn * 128 * NP + grad_codes_bytes(FMT);
     a.stages = stages_for(stageBytes, MAX_STAGES);
-    const int smem = smem_for(stageBytes, a.stages, WEIGHT ? 128 * (a.bn + 4) * 4 : a.splits > 1 ? 128 * a.bn * 4 : 0);
-    const dim3 grid((unsigned) ((a.I + 127) / 128), (unsigned) ((a.N + a.bn - 1) / a.bn), (unsigned) a.splits);
-    return launch_cluster(k_mx_grad<WEIGHT, FMT, DENSE, TD, TO>, grid, DENSE ? GT_DENSE : GT, smem, a.splits, st, mc, md, a);
+    const int smem = smem_for(stageBytes, a.stages, a.splits > 1 ? 128 * (a.bn + 4) * 4 : 0);
+    const dim3 grid((unsigned) (a.splits > 1 ? a.tiles : std::min(a.tiles, sms)), 1, (unsigned) a.splits);
+    return launch_cluster(k_mx_grad<WEIGHT, FMT, DENSE, TD, TO>, grid, GradGroups<(DENSE > 0)>::threads, smem, a.splits, st, mc, md, a);
 }
 
 template <bool WEIGHT, int FMT, class TO>
@@ -685,16 +1107,20 @@ static int grad_common(const char* who, bool weight, void* stream, const void* d
     a.add = add != 0;
     a.vec = (((uintptr_t) dy | (uintptr_t) (ldDy * mx_type_bytes(dyType))) & 15) == 0;
     const bool tma = dyType == QAGG_BF16 && a.vec;
-    const int planes = dyType == QAGG_BF16 ? 1 : dyType == QAGG_F16 ? 2 : 3;
-    const Shape sh = choose_shape((I + 127) / 128, N, (int) ((C + GK - 1) / GK), cfg.numSMs, planes > 1 ? 128 : 256, 64);
+    static const int wide[] = {GRAD_WIDEST, GRAD_WIDEST_DENSE, 64};
+    const Shape sh = choose_shape((I + 127) / 128, N, (int) ((C + GK - 1) / GK), cfg.numSMs, tma ? wide : wide + 1, tma ? 3 : 2, dyType == QAGG_BF16 ? 1 : dyType == QAGG_F16 ? 2 : 3,
+                                  grad_codes_bytes(format), GK * mx_type_bytes(dyType));
     a.bn = sh.bn;
     a.splits = sh.splits;
+    a.tilesM = (int) ((I + 127) / 128);
+    a.tiles = a.tilesM * (int) ((N + a.bn - 1) / a.bn);
+    a.wide = weight ? ((((uintptr_t) out | (uintptr_t) (ldOut * 4)) & 15) == 0) : ((uintptr_t) out & 3) == 0 && (ldOut & 1) == 0;
     alignas(64) CUtensorMap mc, md;
     std::memset(&mc, 0, sizeof(mc));
     std::memset(&md, 0, sizeof(md));
-    if (C > 0 && !codes_map(&mc, codes, I, C, format, format == QAGG_MXFP4 ? 64 : 128, GK, false))
+    if (C > 0 && !codes_map(&mc, codes, I, C, format, format == QAGG_MXFP4 ? 64 : 128, GK))
         return fail(QAGG_ECUDA, std::string(who) + ": tensor map of the codes could not be made");
-    if (C > 0 && tma && !encode_map_tiled(&md, 2, dy, O, T, ldDy * 2, 64, weight ? GK : a.bn, true))
+    if (C > 0 && tma && !encode_map_tiled(&md, 2, dy, O, T, ldDy * 2, 64, weight ? GK : a.bn, 128))
         return fail(QAGG_ECUDA, std::string(who) + ": tensor map of dy could not be made");
     const cudaStream_t st = (cudaStream_t) stream;
     cudaError_t e;
@@ -753,26 +1179,30 @@ int qagg_mx_times(void* stream, const void* w_codes, const void* w_scales, const
     a.O = O;
     a.T = T;
     a.K = K;
-    const Shape sh = choose_shape((O + 127) / 128, T, (int) ((K + TK - 1) / TK), cfg.numSMs, 256, 16);
+    static const int widths[] = {256, 128, 64, 32, 16};
+    const Shape sh = choose_shape((O + 127) / 128, T, (int) ((K + TK - 1) / TK), cfg.numSMs, widths, 5, 1, 128 * (128 + 8), 128 + 8);
     a.bn = sh.bn;
     a.splits = sh.splits;
+    a.tilesM = (int) ((O + 127) / 128);
+    a.tiles = a.tilesM * (int) ((T + a.bn - 1) / a.bn);
+    a.pairs = ((uintptr_t) y & 3) == 0 && (ld_y & 1) == 0;
     const int stageBytes = times_stage_bytes(a.bn);
     a.stages = stages_for(stageBytes, MAX_STAGES);
     const int smem = smem_for(stageBytes, a.stages, a.splits > 1 ? 128 * a.bn * 4 : 0);
     alignas(64) CUtensorMap mw, mx;
     std::memset(&mw, 0, sizeof(mw));
     std::memset(&mx, 0, sizeof(mx));
-    if (K > 0 && (!codes_map(&mw, w_codes, K, O, QAGG_MXFP4, 128, 128, true) || !codes_map(&mx, x_codes, K, T, QAGG_MXFP4, 128, a.bn, true)))
+    if (K > 0 && (!codes_map(&mw, w_codes, K, O, QAGG_MXFP4, 128, 128) || !codes_map(&mx, x_codes, K, T, QAGG_MXFP4, 128, a.bn)))
         return fail(QAGG_ECUDA, "qagg_mx_times: tensor maps of the codes could not be made");
-    const dim3 grid((unsigned) ((O + 127) / 128), (unsigned) ((T + a.bn - 1) / a.bn), (unsigned) a.splits);
+    const dim3 grid((unsigned) (a.splits > 1 ? a.tiles : std::min(a.tiles, cfg.numSMs)), 1, (unsigned) a.splits);
     const cudaStream_t st = (cudaStream_t) stream;
     cudaError_t e;
     if (y_type == QAGG_F32)
-        e = launch_cluster(k_mx_times<float>, grid, GT, smem, a.splits, st, mw, mx, a);
+        e = launch_cluster(k_mx_times<float>, grid, TT, smem, a.splits, st, mw, mx, a);
     else if (y_type == QAGG_F16)
-        e = launch_cluster(k_mx_times<__half>, grid, GT, smem, a.splits, st, mw, mx, a);
+        e = launch_cluster(k_mx_times<__half>, grid, TT, smem, a.splits, st, mw, mx, a);
     else
-        e = launch_cluster(k_mx_times<__nv_bfloat16>, grid, GT, smem, a.splits, st, mw, mx, a);
+        e = launch_cluster(k_mx_times<__nv_bfloat16>, grid, TT, smem, a.splits, st, mw, mx, a);
     return check_cuda(e, "4-bit product kernel launch");
 }
 

@@ -836,7 +836,7 @@ static EncodeTiledFn tensor_map_encoder()
 }
 
 bool encode_map_tiled(void* out128, int elemBytes, const void* base, long long inner, long long outer, long long strideBytes, int boxInner, int boxOuter,
-                      bool swizzle128)
+                      int swizzle)
 {
     EncodeTiledFn enc = tensor_map_encoder();
     if (!enc)
@@ -846,7 +846,7 @@ bool encode_map_tiled(void* out128, int elemBytes, const void* base, long long i
     const cuuint32_t box[2] = {(cuuint32_t) boxInner, (cuuint32_t) boxOuter};
     const cuuint32_t estr[2] = {1, 1};
     return enc(static_cast<CUtensorMap*>(out128), elemBytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims,
-               strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+               strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE,
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

@@ -46,6 +46,15 @@ __device__ __forceinline__ void tc_wait(unsigned long long* bar, unsigned parity
     }
 }
 
+// True in one lane of a converged warp.  The tensor cores' instructions take uniform registers; behind this (rather than lane == 0)
+// the compiler knows their operands to be uniform.  With lane == 0 each instruction cost its thread about 150 cycles.
+__device__ __forceinline__ bool elect_one()
+{
+    unsigned ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+    return ok != 0;
+}
+
 // ---- copies -----------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void tma_load_2d(unsigned dst, const void* tmap, int x0, int x1, unsigned long long* bar)
 {
@@ -84,24 +93,42 @@ __device__ __forceinline__ void tc_fence_after()
 {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
-// 32 columns of this warp's 32 lanes <-> 32 registers
-__device__ __forceinline__ void tmem_load32(unsigned addr, unsigned (&r)[32])
+// 16 columns of this warp's 32 lanes: register j of lane l is column j
+__device__ __forceinline__ void tmem_load16(unsigned addr, unsigned (&r)[16])
 {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-                   "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-                   "=r"(r[31])
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(addr));
+}
+__device__ __forceinline__ void tmem_load_wait()
+{
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void tmem_store16(unsigned addr, const unsigned (&r)[16])
+// 32 columns of 16 lanes: registers 4 g, 4 g + 1 are columns 8 g + 2 (l % 4), + 1 of lane l / 4, registers 4 g + 2, + 3 those of lane l / 4 + 8
+__device__ __forceinline__ void tmem_store_16x256b(unsigned addr, const unsigned (&r)[16])
 {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr), "r"(r[0]),
+    asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr), "r"(r[0]),
                  "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
                  "r"(r[14]), "r"(r[15])
                  : "memory");
+}
+// Two 16 x 16 matrices of bytes from shared memory, transposed.  Lanes 0-15 give the rows' addresses of the first, 16-31 of the second.
+// Registers 0 and 1 (first matrix), 2 and 3: bytes of column l / 4 (second register: + 8), rows 4 (l % 4) .. + 3.
+__device__ __forceinline__ void ldmatrix_trans_b8(unsigned addr, unsigned (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// registers per thread of this warp's group of four warps, whose warps all get here
+template <int N>
+__device__ __forceinline__ void registers_up()
+{
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void registers_down()
+{
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 __device__ __forceinline__ void tmem_store_wait()
 {
@@ -167,10 +194,14 @@ __device__ __forceinline__ void cluster_sync()
 {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float4 cluster_load4(unsigned addr, unsigned rank)
+__device__ __forceinline__ unsigned cluster_address(unsigned addr, unsigned rank)
 {
     unsigned remote;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+    return remote;
+}
+__device__ __forceinline__ float4 cluster_load4(unsigned remote)
+{
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
     return v;

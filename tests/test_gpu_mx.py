@@ -165,7 +165,7 @@ def test_offsets_beyond_32_bits(lib):
 
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("O,T,K,pad", [(128, 16, 256, 0), (1, 1, 1, 0), (128, 1, 32, 0), (129, 1, 2048, 0), (2048, 1, 2048, 0), (100, 3, 64, 5), (132, 17, 512, 0),
-                                       (512, 33, 363, 8), (300, 129, 429, 1), (256, 256, 1024, 0), (2048, 300, 429, 0), (520, 511, 96, 0), (1000, 1000, 1000, 0)])
+                                       (512, 33, 363, 8), (300, 129, 429, 1), (256, 256, 1024, 0), (2048, 300, 429, 0), (520, 511, 96, 0), (1000, 1000, 1000, 0), (2200, 2500, 900, 0)])
 def test_times(lib, O, T, K, pad, t):
     rng = np.random.default_rng(O + T + K)
     (wc, ws), w = packed(rng, O, K, mx_util.FP4, 0.05)
@@ -246,6 +246,26 @@ def test_input_grad(lib, O, I, T, pad, offset, t, fmt):
         lib.mx_check(stream())
         check(dx, want, mags, planes * O / 16, t2, "input gradient")
         untouched(flat, dx, pad, offset)
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("O,I,T", [(2048, 1100, 2100), (2049, 1100, 2100)])
+def test_more_tiles_than_sms(lib, O, I, T, t):
+    """Several tiles per CTA, with and without 16-byte columns of dy."""
+    rng = np.random.default_rng(O)
+    _, d, dy = dense(rng, T, O, t, 0, 0, 1e-2)
+    planes = {"bf16": 1, "f16": 2, "f32": 3}[t]
+    (xc, xs), x = packed(rng, T, I, mx_util.INT8)
+    _, dw = room(I, O, "f32")
+    lib.mx_weight_grad(d.data_ptr(), code(lib, t), O, xc.data_ptr(), xs.data_ptr(), 8, dw.data_ptr(), O, I, T, False, stream())
+    lib.mx_check(stream())
+    check(dw, x.T @ dy, np.abs(x).T @ np.abs(dy), planes * T / 16, "f32", "weight gradient")
+    (wc, ws), w = packed(rng, O, I, mx_util.FP4, 0.05)
+    for t2 in dict.fromkeys((t, "f32")):
+        _, dx = room(T, I, t2)
+        lib.mx_input_grad(d.data_ptr(), code(lib, t), O, wc.data_ptr(), ws.data_ptr(), 4, dx.data_ptr(), code(lib, t2), I, O, I, T, stream())
+        lib.mx_check(stream())
+        check(dx, dy @ w, np.abs(dy) @ np.abs(w), planes * O / 16, t2, "input gradient")
 
 
 def test_gradients_of_nothing(lib):
