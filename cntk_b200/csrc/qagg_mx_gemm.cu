@@ -82,25 +82,25 @@ __device__ __forceinline__ void drain_copies(GemmBars* bars, long long issued, i
             ;
 }
 
-// First warp: barriers.  The copies may start right after this, before the CTA has met.
+// First warp, all lanes: barriers.  The copies may start right after this, before the CTA has met.
 __device__ __forceinline__ void init_barriers(GemmBars* bars, int stages, int convCount, int denseCount, int resultWarps)
 {
-    for (int s = 0; s < stages; ++s)
+    const int lane = threadIdx.x & 31, s = lane >> 2;
+    if (s < stages)
+        mbar_init(lane & 2 ? (lane & 1 ? &bars->empty[s] : &bars->dense[s]) : (lane & 1 ? &bars->conv[s] : &bars->full[s]),
+                  (lane & 3) == 1 ? convCount : (lane & 3) == 2 ? denseCount : 1);
+    if (lane < 2)
     {
-        mbar_init(&bars->full[s], 1);
-        mbar_init(&bars->conv[s], convCount);
-        mbar_init(&bars->dense[s], denseCount);
-        mbar_init(&bars->empty[s], 1);
+        mbar_init(&bars->ready[lane], 1);
+        mbar_init(&bars->taken[lane], resultWarps);
     }
-    for (int b = 0; b < 2; ++b)
-    {
-        mbar_init(&bars->ready[b], 1);
-        mbar_init(&bars->taken[b], resultWarps);
-    }
-    bars->broken = 0;
+    if (lane == 0)
+        bars->broken = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_shared();
+    __syncwarp();
 }
+static_assert(MAX_STAGES <= 8, "four lanes of a warp per stage");
 
 // ---- results ------------------------------------------------------------------------------------------------------------------
 
@@ -119,7 +119,7 @@ __device__ __forceinline__ unsigned pack2(float a, float b, __nv_bfloat16*)
 }
 
 // `cols` columns (a multiple of 16) of a finished chain, set or added to the registers.
-template <int ACC>
+template <bool PAIR, int ACC>
 __device__ __forceinline__ void take_chain(GemmBars* bars, int buf, unsigned par, unsigned tmem, int cols, bool firstChain, float (&acc)[ACC])
 {
     tc_wait(&bars->ready[buf], par, &bars->broken, &g_mxStatus);
@@ -139,7 +139,12 @@ __device__ __forceinline__ void take_chain(GemmBars* bars, int buf, unsigned par
     tc_fence_before();
     __syncwarp();
     if ((threadIdx.x & 31) == 0)
-        mbar_arrive(&bars->taken[buf]);
+    {
+        if constexpr (PAIR)
+            mbar_arrive_remote(&bars->taken[buf], 0);
+        else
+            mbar_arrive(&bars->taken[buf]);
+    }
 }
 // Which accumulator a chain uses, and the parity of its barriers' phase.
 struct Chains
@@ -305,6 +310,7 @@ struct TimesArgs
 };
 
 constexpr int TT = 384;  // copy, product, allocating and spare warp; eight result warps
+constexpr int TIMES_NARROW = 32;
 constexpr int TK = 256;  // contraction values per stage: 128 bytes of codes
 
 
@@ -313,7 +319,9 @@ __host__ __device__ inline int times_stage_bytes(int bn)
     return 128 * 128 + bn * 128 + 1024 + (bn > 128 ? 2048 : 1024);
 }
 
-template <class T>
+// ACC: most columns of the tile that one result warp holds.  The narrow tiles of few tokens have a kernel of their own, whose results are
+// a quarter of the code: a launch that lasts 3 us feels the instruction fetches (128: 1400 cycles to put the sums down).
+template <class T, int ACC>
 __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapX, const TimesArgs a)
 {
     extern __shared__ unsigned char dyn[];
@@ -331,28 +339,38 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
     constexpr unsigned SIDE = 256;     // block scales: 24 columns a stage
     constexpr int CHAIN_STEPS = (sizeof(T) == 4 ? CHAIN : CHAIN_16BIT) / 4;
 
-    auto copy_step = [&](int tile, int i, int s) {
-        const long long m0 = (long long) (tile % a.tilesM) * 128, n0 = (long long) (tile / a.tilesM) * bn;
-        const int rowsX = bn > 128 && n0 + 128 < a.T ? 2 : 1;
-        const unsigned at = smem_addr(stage0) + s * stageBytes;
+    // The copying thread's time per step counts: what depends on the tile alone is worked out once per tile.
+    struct Source
+    {
+        int m0, n0, rowsX;
+        const unsigned char *scaleW, *scaleX;
+    };
+    auto source_of = [&](int tile) {
+        const int m = tile % a.tilesM, n0 = tile / a.tilesM * bn;
+        return Source{m * 128, n0, bn > 128 && n0 + 128 < a.T ? 2 : 1, a.scaleW + (long long) m * chunks * 512, a.scaleX + (long long) (n0 / 128) * chunks * 512};
+    };
+    auto copy_step = [&](const Source& src, int i, int s) {
+        const unsigned at = smem_addr(stage0) + s * stageBytes, sw = at + 16384 + bn * 128;
         const int k = first + i;
-        const unsigned nch = chunks - 2LL * k < 2 ? 1 : 2;
-        mbar_arrive_expect_tx(&bars.full[s], 128 * 128 + bn * 128 + nch * 512 * (1 + rowsX));
-        tma_load_2d(at, &mapW, k * 128, (int) m0, &bars.full[s]);
-        tma_load_2d(at + 16384, &mapX, k * 128, (int) n0, &bars.full[s]);
-        const unsigned sw = at + 16384 + bn * 128;
-        bulk_load(sw, a.scaleW + ((m0 / 128) * chunks + 2LL * k) * 512, nch * 512, &bars.full[s]);
-        for (int r = 0; r < rowsX; ++r)
-            bulk_load(sw + 1024 + r * 1024, a.scaleX + ((n0 / 128 + r) * chunks + 2LL * k) * 512, nch * 512, &bars.full[s]);
+        const unsigned bytes = chunks - 2 * k < 2 ? 512 : 1024;
+        unsigned long long* full = &bars.full[s];
+        mbar_arrive_expect_tx(full, 128 * 128 + bn * 128 + bytes * (1 + src.rowsX));
+        tma_load_2d(at, &mapW, k * 128, src.m0, full);
+        tma_load_2d(at + 16384, &mapX, k * 128, src.n0, full);
+        bulk_load(sw, src.scaleW + k * 1024LL, bytes, full);
+        bulk_load(sw + 1024, src.scaleX + k * 1024LL, bytes, full);
+        if (src.rowsX == 2)
+            bulk_load(sw + 2048, src.scaleX + (chunks + 2LL * k) * 512, bytes, full);
     };
     int early = 0; // steps of the first tile whose copies start before the CTA has met
     if (warp == 0)
     {
+        init_barriers(&bars, S, 1, 1, resultWarps);
         if (elect_one())
         {
-            init_barriers(&bars, S, 1, 1, resultWarps);
+            const Source src = source_of(blockIdx.x);
             for (; early < count && early < S; ++early)
-                copy_step(blockIdx.x, early, early);
+                copy_step(src, early, early);
         }
         early = count < S ? count : S;
         __syncwarp();
@@ -373,6 +391,8 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
                 ring.next(S);
             long long issued = early;
             for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
+            {
+                const Source src = source_of(tile);
                 for (int i = tile == (int) blockIdx.x ? early : 0; i < count; ++i, ++issued)
                 {
                     if (issued >= S)
@@ -380,13 +400,13 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
                     if (*reinterpret_cast<volatile unsigned*>(&bars.broken))
                     {
                         drain_copies(&bars, issued, S);
-                        i = count;
                         tile = a.tiles;
                         break;
                     }
-                    copy_step(tile, i, ring.s);
+                    copy_step(src, i, ring.s);
                     ring.next(S);
                 }
+            }
         }
     }
     else if (warp == 1)
@@ -459,13 +479,13 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
             for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
             {
                 const long long m0 = (long long) (tile % a.tilesM) * 128, n0 = (long long) (tile / a.tilesM) * bn;
-                float acc[128];
+                float acc[ACC];
 #pragma unroll
-                for (int j = 0; j < 128; ++j)
+                for (int j = 0; j < ACC; ++j)
                     acc[j] = 0.0f;
                 const float bias = a.bias && a.splits == 1 && m0 + m < a.O ? a.bias[m0 + m] : 0.0f;
                 for (int i = 0; i < count; i += CHAIN_STEPS, chain.next(bufs))
-                    take_chain(&bars, chain.buf, chain.par, mine + chain.buf * 128, cols, i == 0, acc);
+                    take_chain<false>(&bars, chain.buf, chain.par, mine + chain.buf * 128, cols, i == 0, acc);
                 if (a.splits > 1)
                     put_partial<false>(reinterpret_cast<float*>(stage0), bn, m, half * 128, cols, acc);
                 else
@@ -506,24 +526,34 @@ constexpr int GK = 64; // contraction values per stage
 // Threads, in groups of four warps: copy / product / allocating / spare; expanding; result; with a dense operand that the copy engine
 // cannot take, one group less of the second and third kind and four of loaders.  The threads are launched with as many registers
 // each as the SM has for all of them, and redistribute them.
+// PAIR: two CTAs make a 256 x 256 tile together, each with 128 rows of the packed operand and half of dy's columns, so that each brings
+// 24 KB (int8; fp4 20) for 512 cycles of products where a CTA by itself brings 32 (28) for 384: copies from L2, at some 46
+// bytes a cycle, are what bounds these kernels.
 // Tensor memory: two accumulators of 192 columns and four expanded steps of 32, or, tiles being 128 wide with loaders, two of 128
-// and eight.  A 192-wide tile reads 6 % more per product than one of 256, which would leave room for one accumulator.
-constexpr int GRAD_WIDEST = 192, GRAD_WIDEST_DENSE = 128;
-template <bool DENSE>
+// and eight.  A 192-wide tile reads 6 % more per product than one of 256, which would leave room for one accumulator.  A pair has one
+// of 256 columns, and eight expanded steps.
+constexpr int GRAD_WIDEST = 192, GRAD_WIDEST_DENSE = 128, GRAD_PAIR = 256;
+template <bool DENSE, bool PAIR>
 struct GradGroups
 {
-    static constexpr int expand = DENSE ? 1 : 3, result = DENSE ? 1 : 2, load = DENSE ? 4 : 0;
+    static constexpr int expand = DENSE ? 1 : PAIR ? 2 : 3, result = DENSE ? 1 : 2, load = DENSE ? 4 : 0;
     static constexpr int firstExpand = 4, firstResult = firstExpand + 4 * expand, firstLoad = firstResult + 4 * result;
     static constexpr int threads = 128 * (1 + expand + result + load);
-    static constexpr int regsLaunch = DENSE ? 72 : 80; // 65536 / threads, a multiple of 8
-    static constexpr int regsMisc = DENSE ? 40 : 56, regsExpand = 56, regsResult = DENSE ? 152 : 128, regsLoad = 64;
+    static constexpr int regsLaunch = DENSE ? 72 : PAIR ? 96 : 80; // 65536 / threads, a multiple of 8
+    static constexpr int regsMisc = DENSE ? 40 : PAIR ? 48 : 56, regsExpand = PAIR ? 64 : 56, regsResult = DENSE || PAIR ? 152 : 128, regsLoad = 64;
     static_assert(regsLaunch * threads <= 65536 && 128 * (regsMisc + regsExpand * expand + regsResult * result + regsLoad * load) <= regsLaunch * threads, "registers");
+    static constexpr int widest = DENSE ? GRAD_WIDEST_DENSE : PAIR ? GRAD_PAIR : GRAD_WIDEST;
+    static constexpr int accumulators = PAIR ? 1 : 2;
+    static constexpr unsigned side = accumulators * widest;      // first column behind the accumulators
+    static constexpr int slots = (int) (TMEM_COLS - side) / 32; // expanded steps in tensor memory
 };
 
+// packed part of a stage: 64 contraction values x 128 rows of codes, and the scale tile they lie in (128 values x 128 rows)
 __host__ __device__ inline int grad_codes_bytes(int format)
 {
     return GK * (format == QAGG_MXFP4 ? 64 : 128);
 }
+constexpr int GRAD_SCALE_BYTES = 512, GRAD_SCALE_ROOM = 1024; // stages stay multiples of 1024 bytes
 
 // Codes to bf16.  v: four codes of one row (int8), or four bytes with one code of an even and one of an odd row each (fp4), from
 // contraction values k..k+3; pair 0 is (k, k + 1), pair 1 (k + 2, k + 3).
@@ -603,65 +633,84 @@ __device__ __forceinline__ bool any_special(const Raw8<T>& raw)
 // WEIGHT: dw, lanes = i, columns = o, contraction over the tokens; the dense operand is MN-major (o runs fastest).
 // otherwise: dx, lanes = i, columns = t, contraction over o; the dense operand is K-major.
 // DENSE 0: dy is bf16 and the copy engine can take it.  DENSE 1..3: that many bf16 planes, made by loader warps from TD.
-template <bool WEIGHT, int FMT, int DENSE, class TD, class TO>
-__global__ void __launch_bounds__(GradGroups<(DENSE > 0)>::threads, 1) k_mx_grad(const __grid_constant__ CUtensorMap mapCodes, const __grid_constant__ CUtensorMap mapDy, const GradArgs a)
+template <bool WEIGHT, int FMT, int DENSE, bool PAIR, class TD, class TO>
+__global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_mx_grad(const __grid_constant__ CUtensorMap mapCodes, const __grid_constant__ CUtensorMap mapDy, const GradArgs a)
 {
-    using G = GradGroups<(DENSE > 0)>;
+    using G = GradGroups<(DENSE > 0), PAIR>;
+    static_assert(!(PAIR && DENSE), "pairs bring dy through the copy engine");
     constexpr int NP = DENSE ? DENSE : 1;
     constexpr int CHAIN_STEPS = (sizeof(TO) == 4 ? CHAIN : CHAIN_16BIT) / 4 / NP;
-    constexpr int WIDEST = DENSE ? GRAD_WIDEST_DENSE : GRAD_WIDEST;
-    constexpr unsigned SIDE = 2 * WIDEST;
-    constexpr int SLOTS = (TMEM_COLS - SIDE) / 32; // expanded steps in tensor memory
+    constexpr int WIDEST = G::widest, SLOTS = G::slots, BUFS = G::accumulators;
     extern __shared__ unsigned char dyn[];
     __shared__ GemmBars bars;
     __shared__ __align__(16) unsigned short scaleRows[4 * G::expand][GK]; // per expanding warp: its block's multipliers for one step
     unsigned char* stage0 = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t) 1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int bn = a.bn, S = a.stages;
-    const int denseBytes = bn * 128 * NP;
-    const int stageBytes = denseBytes + grad_codes_bytes(FMT);
+    const int share = PAIR ? bn / 2 : bn; // columns of dy that this CTA brings
+    const int denseBytes = share * 128 * NP;
+    const int stageBytes = denseBytes + grad_codes_bytes(FMT) + GRAD_SCALE_ROOM;
     const int steps = (int) ((a.C + GK - 1) / GK);
-    const int rank = a.splits > 1 ? (int) cluster_rank() : 0;
-    int first, count;
-    split_range(steps, rank, a.splits, first, count);
+    const int rank = PAIR || a.splits > 1 ? (int) cluster_rank() : 0;
+    int first = 0, count = steps;
+    if (!PAIR)
+        split_range(steps, rank, a.splits, first, count);
+    const int firstTile = PAIR ? blockIdx.x >> 1 : blockIdx.x, tileStep = PAIR ? gridDim.x >> 1 : gridDim.x;
     constexpr int resultWarps = 4 * G::result;
-    auto tile_m0 = [&](int tile) { return (long long) (tile % a.tilesM) * 128; };
+    auto tile_m0 = [&](int tile) { return (long long) (tile % a.tilesM) * (PAIR ? 256 : 128) + (PAIR ? rank * 128 : 0); };
     auto tile_n0 = [&](int tile) { return (long long) (tile / a.tilesM) * bn; };
 
-    auto copy_step = [&](int tile, int i, int s) {
-        const int m0 = (int) tile_m0(tile), n0 = (int) tile_n0(tile);
+    // what a copied step needs, worked out once per tile
+    struct Source
+    {
+        int codes, n0;
+        const unsigned char* scales;
+    };
+    const long long scaleRow = mx_scale_tiles(a.I) * GRAD_SCALE_BYTES; // from 128 contraction values to the next
+    auto source_of = [&](int tile) {
+        const int m0 = (int) tile_m0(tile);
+        // (a CTA of a pair may have no rows of the packed matrix: codes outside read as zero, scales are taken from the last rows)
+        const long long rowTile = m0 < a.I ? m0 / 128 : (a.I - 1) / 128;
+        return Source{FMT == QAGG_MXFP4 ? m0 / 2 : m0, (int) tile_n0(tile) + (PAIR ? rank * share : 0), a.scales + rowTile * GRAD_SCALE_BYTES};
+    };
+    auto copy_step = [&](const Source& src, int i, int s) {
         const unsigned at = smem_addr(stage0) + s * stageBytes;
         const int k0 = (first + i) * GK;
-        mbar_arrive_expect_tx(&bars.full[s], grad_codes_bytes(FMT) + (DENSE ? 0 : denseBytes));
-        tma_load_2d(at + denseBytes, &mapCodes, FMT == QAGG_MXFP4 ? m0 / 2 : m0, k0, &bars.full[s]);
+        unsigned long long* full = &bars.full[s];
+        mbar_arrive_expect_tx(full, grad_codes_bytes(FMT) + GRAD_SCALE_BYTES + (DENSE ? 0 : denseBytes));
+        tma_load_2d(at + denseBytes, &mapCodes, src.codes, k0, full);
+        bulk_load(at + denseBytes + grad_codes_bytes(FMT), src.scales + (k0 >> 7) * scaleRow, GRAD_SCALE_BYTES, full);
         if constexpr (DENSE == 0)
         {
             if constexpr (WEIGHT)
-                for (int n = 0; n < bn; n += 64)
-                    tma_load_2d(at + n * 128, &mapDy, n0 + n, k0, &bars.full[s]);
+                for (int n = 0; n < share; n += 64)
+                    tma_load_2d(at + n * 128, &mapDy, src.n0 + n, k0, full);
             else
-                tma_load_2d(at, &mapDy, k0, n0, &bars.full[s]);
+                tma_load_2d(at, &mapDy, k0, src.n0, full);
         }
     };
     int early = 0; // steps of the first tile whose copies start before the CTA has met
     if (warp == 0)
     {
+        init_barriers(&bars, S, PAIR ? 8 : 4, 4 * G::load, PAIR ? 2 * resultWarps : resultWarps);
         if (elect_one())
         {
-            init_barriers(&bars, S, 4, 4 * G::load, resultWarps);
+            const Source src = source_of(firstTile);
             for (; early < count && early < S; ++early)
-                copy_step(blockIdx.x, early, early);
+                copy_step(src, early, early);
         }
         early = count < S ? count : S;
         __syncwarp();
     }
     if (warp == 2)
-        tmem_alloc(&bars.tmem, TMEM_COLS);
+        tmem_alloc<PAIR>(&bars.tmem, TMEM_COLS);
     tc_fence_before();
     __syncthreads();
+    if (PAIR)
+        cluster_sync(); // the other CTA's barriers exist
     tc_fence_after();
     const unsigned tm = bars.tmem;
-    const unsigned tmA = tm + SIDE;
+    const unsigned tmA = tm + G::side;
 
     if (warp < 4)
     {
@@ -672,8 +721,10 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0)>::threads, 1) k_mx_grad
             for (int i = 0; i < early; ++i)
                 ring.next(S);
             long long issued = early;
-            for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
-                for (int i = tile == (int) blockIdx.x ? early : 0; i < count; ++i, ++issued)
+            for (int tile = firstTile; tile < a.tiles; tile += tileStep)
+            {
+                const Source src = source_of(tile);
+                for (int i = tile == firstTile ? early : 0; i < count; ++i, ++issued)
                 {
                     if (issued >= S)
                         tc_wait(&bars.empty[ring.s], ring.par ^ 1, &bars.broken, &g_mxStatus);
@@ -683,20 +734,21 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0)>::threads, 1) k_mx_grad
                         tile = a.tiles;
                         break;
                     }
-                    copy_step(tile, i, ring.s);
+                    copy_step(src, i, ring.s);
                     ring.next(S);
                 }
+            }
         }
-        else if (warp == 1 && elect_one())
+        else if (warp == 1 && (!PAIR || rank == 0) && elect_one())
         {
             Ring ring;
             Chains chain;
             bool fresh = true; // accumulators that no chain has used
             int slot = 0;
-            const unsigned idesc = idesc_bf16(bn, WEIGHT);
+            const unsigned idesc = idesc_bf16(bn, WEIGHT, PAIR ? 256 : 128);
             const unsigned long long d0 = WEIGHT ? smem_desc(smem_addr(stage0), 8192, 1024, SWIZZLE_128B) : smem_desc(smem_addr(stage0), 16, 1024, SWIZZLE_128B);
             constexpr unsigned KSTEP = (WEIGHT ? 2048 : 32) >> 4;
-            for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
+            for (int tile = firstTile; tile < a.tiles; tile += tileStep)
             {
                 int inChain = 0;
                 for (int i = 0; i < count; ++i)
@@ -715,13 +767,22 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0)>::threads, 1) k_mx_grad
                     for (int p = 0; p < NP; ++p)
 #pragma unroll
                         for (int j = 0; j < GK / 16; ++j)
-                            mma_bf16_ts(acc, ta + j * 8, d + p * (bn * 128 >> 4) + j * KSTEP, idesc, inChain > 0 || p + j > 0);
-                    tc_commit(&bars.empty[ring.s]);
+                            if constexpr (PAIR)
+                                mma_bf16_ts_pair(acc, ta + j * 8, d + j * KSTEP, idesc, inChain > 0 || j > 0);
+                            else
+                                mma_bf16_ts(acc, ta + j * 8, d + p * (bn * 128 >> 4) + j * KSTEP, idesc, inChain > 0 || p + j > 0);
+                    if constexpr (PAIR)
+                        tc_commit_pair(&bars.empty[ring.s]);
+                    else
+                        tc_commit(&bars.empty[ring.s]);
                     ring.next(S);
                     if (++inChain == CHAIN_STEPS || i + 1 == count)
                     {
-                        tc_commit(&bars.ready[chain.buf]);
-                        chain.next(2);
+                        if constexpr (PAIR)
+                            tc_commit_pair(&bars.ready[chain.buf]);
+                        else
+                            tc_commit(&bars.ready[chain.buf]);
+                        chain.next(BUFS);
                         fresh = fresh && chain.buf != 0;
                         inChain = 0;
                     }
@@ -737,7 +798,7 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0)>::threads, 1) k_mx_grad
         // store to tensor memory takes pairs of contraction values.  With fp4 that puts row 16 h + 2 b + o of the block on lane
         // 16 h + 8 o + b; the result warps know.  Several groups of warps take the steps in turn.
         const int quad = warp & 3, group = (warp - G::firstExpand) >> 2;
-        const long long tileRow = mx_scale_tiles(a.I) * 512;
+        const unsigned char* scaleAt = stage0 + denseBytes + grad_codes_bytes(FMT) + lane * 16 + quad; // of contraction value `lane` of a tile
         unsigned short* mult = scaleRows[warp - G::firstExpand];
         // rows of the code tile are 128 (fp4: 64) bytes, their 16-byte pieces swizzled by the copy
         constexpr int ROW = FMT == QAGG_MXFP4 ? 64 : 128;
@@ -767,92 +828,65 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0)>::threads, 1) k_mx_grad
                 oldPar ^= 1;
             }
         };
-        for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
+        for (int tile = firstTile; tile < a.tiles; tile += tileStep)
         {
-            const unsigned char* mine = a.scales + tile_m0(tile) / 128 * 512 + lane * 16 + quad;
-            auto fetch = [&](int i, unsigned& b0, unsigned& b1) { // the scale tiles cover whole groups of 128 columns
-                const unsigned k = (unsigned) (first + i) * GK;
-                const unsigned char* p = mine + (long long) (k / 128) * tileRow + (k & 64) / 8;
-                b0 = p[0];
-                b1 = p[4];
-            };
-            unsigned b0 = 0, b1 = 0;
             int i = 0;
             for (; i < count && n % G::expand != group; ++i) // steps of the other groups
                 advance(1);
-            if (i < count)
-                fetch(i, b0, b1);
             for (; i < count; i += G::expand)
             {
-                __syncwarp();
-                mult[lane] = (unsigned short) scale_bf16<FMT>(b0);
-                mult[lane + 32] = (unsigned short) scale_bf16<FMT>(b1);
-                if (i + G::expand < count)
-                    fetch(i + G::expand, b0, b1);
-                __syncwarp();
                 tc_wait(&bars.full[stage], par, &bars.broken, &g_mxStatus);
+                __syncwarp(); // also: the multipliers of the previous step have been read
+                const unsigned off = stage * stageBytes;
+                // piece g of a block half is 16 contraction values: two registers
+                constexpr int HALVES = FMT == QAGG_MXINT8 ? 2 : 1;
+                unsigned c[HALVES][8];
+#pragma unroll
+                for (int h = 0; h < HALVES; ++h)
+                {
+                    ldmatrix_trans_b8(rowAt[h] + off, reinterpret_cast<unsigned(&)[4]>(c[h][0]));
+                    ldmatrix_trans_b8(rowAt[h] + off + 32 * ROW, reinterpret_cast<unsigned(&)[4]>(c[h][4]));
+                }
+                const unsigned char* sb = scaleAt + off + ((first + i) & 1) * 8;
+                mult[lane] = (unsigned short) scale_bf16<FMT>(sb[0]);
+                mult[lane + 32] = (unsigned short) scale_bf16<FMT>(sb[4]);
                 __syncwarp();
+                uint2 sc[4]; // multipliers of contraction values 16 g + 4 (lane % 4) .. + 3
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    sc[g] = *reinterpret_cast<const uint2*>(mult + 16 * g + 4 * (lane & 3));
                 if (S > SLOTS && n >= SLOTS)
                 {
                     tc_wait(&bars.empty[oldStage], oldPar, &bars.broken, &g_mxStatus);
                     __syncwarp();
                 }
                 tc_fence_after();
-                const unsigned off = stage * stageBytes;
                 const unsigned to = tmA + ((unsigned) (quad * 32) << 16) + slot * 32;
-                uint2 sc[4]; // multipliers of contraction values 16 g + 4 (lane % 4) .. + 3
 #pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    sc[g] = *reinterpret_cast<const uint2*>(mult + 16 * g + 4 * (lane & 3));
-                // piece g of a block half is 16 contraction values: two registers
-                if constexpr (FMT == QAGG_MXINT8)
+                for (int h = 0; h < 2; ++h)
                 {
-                    unsigned c[2][8];
+                    unsigned r[16];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                    {
-                        ldmatrix_trans_b8(rowAt[h] + off, reinterpret_cast<unsigned(&)[4]>(c[h][0]));
-                        ldmatrix_trans_b8(rowAt[h] + off + 32 * ROW, reinterpret_cast<unsigned(&)[4]>(c[h][4]));
-                    }
+                    for (int g = 0; g < 4; ++g)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                    {
-                        unsigned r[16];
-#pragma unroll
-                        for (int g = 0; g < 4; ++g)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                            {
-                                r[4 * g + 2 * e] = expand_int8(c[h][2 * g + e], 0, sc[g].x);
-                                r[4 * g + 2 * e + 1] = expand_int8(c[h][2 * g + e], 1, sc[g].y);
-                            }
-                        tmem_store_16x256b(to + ((unsigned) (h * 16) << 16), r);
-                    }
-                }
-                else
-                {
-                    unsigned c[8], r[16];
-                    ldmatrix_trans_b8(rowAt[0] + off, reinterpret_cast<unsigned(&)[4]>(c[0]));
-                    ldmatrix_trans_b8(rowAt[0] + off + 32 * ROW, reinterpret_cast<unsigned(&)[4]>(c[4]));
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                    {
-#pragma unroll
-                        for (int g = 0; g < 4; ++g)
-#pragma unroll
-                            for (int o = 0; o < 2; ++o)
-                            {
-                                r[4 * g + 2 * o] = expand_fp4(c[2 * g + h], 0, o, sc[g].x);
-                                r[4 * g + 2 * o + 1] = expand_fp4(c[2 * g + h], 1, o, sc[g].y);
-                            }
-                        tmem_store_16x256b(to + ((unsigned) (h * 16) << 16), r);
-                    }
+                        for (int e = 0; e < 2; ++e) // rows l / 4, l / 4 + 8 of the half
+                        {
+                            const unsigned v = FMT == QAGG_MXINT8 ? c[h % HALVES][2 * g + e] : c[0][2 * g + h];
+                            r[4 * g + 2 * e] = FMT == QAGG_MXINT8 ? expand_int8(v, 0, sc[g].x) : expand_fp4(v, 0, e, sc[g].x);
+                            r[4 * g + 2 * e + 1] = FMT == QAGG_MXINT8 ? expand_int8(v, 1, sc[g].y) : expand_fp4(v, 1, e, sc[g].y);
+                        }
+                    tmem_store_16x256b(to + ((unsigned) (h * 16) << 16), r);
                 }
                 tmem_store_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0)
-                    mbar_arrive(&bars.conv[stage]);
+                {
+                    if constexpr (PAIR)
+                        mbar_arrive_remote(&bars.conv[stage], 0);
+                    else
+                        mbar_arrive(&bars.conv[stage]);
+                }
                 advance(min(G::expand, count - i));
             }
         }
@@ -866,7 +900,7 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0)>::threads, 1) k_mx_grad
             const unsigned mine = tm + ((unsigned) (quad * 32) << 16) + half * cols;
             const int m = quad * 32 + (FMT == QAGG_MXFP4 ? (lane & 16) + 2 * (lane & 7) + ((lane >> 3) & 1) : lane);
             Chains chain;
-            for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
+            for (int tile = firstTile; tile < a.tiles; tile += tileStep)
             {
                 const long long m0 = tile_m0(tile), n0 = tile_n0(tile);
                 constexpr int ACC = WIDEST / G::result;
@@ -874,9 +908,9 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0)>::threads, 1) k_mx_grad
 #pragma unroll
                 for (int j = 0; j < ACC; ++j)
                     acc[j] = 0.0f;
-                for (int i = 0; i < count; i += CHAIN_STEPS, chain.next(2))
-                    take_chain(&bars, chain.buf, chain.par, mine + chain.buf * WIDEST, cols, i == 0, acc);
-                if (a.splits > 1)
+                for (int i = 0; i < count; i += CHAIN_STEPS, chain.next(BUFS))
+                    take_chain<PAIR>(&bars, chain.buf, chain.par, mine + chain.buf * WIDEST, cols, i == 0, acc);
+                if (!PAIR && a.splits > 1)
                     put_partial<WEIGHT>(reinterpret_cast<float*>(stage0), bn, m, half * cols, cols, acc);
                 else if constexpr (WEIGHT)
                     write_row((float*) a.out, a.ld, m0 + m, a.I, n0 + half * cols, a.N, cols, acc, a.add != 0, a.wide != 0);
@@ -897,7 +931,7 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0)>::threads, 1) k_mx_grad
         {
             Raw8<TD> raw[UNITS];
         };
-        int nextTile = blockIdx.x, nextStep = 0;
+        int nextTile = firstTile, nextStep = 0;
         auto fetch = [&](Step& st) { // the next step that this CTA has
             if (nextTile >= a.tiles || count == 0)
                 return;
@@ -915,7 +949,7 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0)>::threads, 1) k_mx_grad
             if (++nextStep == count)
             {
                 nextStep = 0;
-                nextTile += gridDim.x;
+                nextTile += tileStep;
             }
         };
         Ring ring;
@@ -952,7 +986,7 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0)>::threads, 1) k_mx_grad
         Step even, odd;
         fetch(even);
         fetch(odd);
-        const long long mySteps = (int) blockIdx.x < a.tiles ? (long long) ((a.tiles - 1 - (int) blockIdx.x) / (int) gridDim.x + 1) * count : 0;
+        const long long mySteps = firstTile < a.tiles ? (long long) ((a.tiles - 1 - firstTile) / tileStep + 1) * count : 0;
         for (long long n = 0; n < mySteps; n += 2)
         {
             put_step(even);
@@ -965,13 +999,15 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0)>::threads, 1) k_mx_grad
         }
     }
     __syncwarp();
-    if (a.splits > 1) // one tile per cluster
+    if (!PAIR && a.splits > 1) // one tile per cluster
         reduce_cluster<WEIGHT, TO>(reinterpret_cast<float*>(stage0), a.splits, rank, bn, (TO*) a.out, a.ld, tile_m0(blockIdx.x), a.I, tile_n0(blockIdx.x), a.N, nullptr,
                                    a.add != 0);
     tc_fence_before();
+    if (PAIR)
+        cluster_sync(); // neither goes while the other may still arrive at its barriers or use its memory
     __syncthreads();
     if (warp == 2)
-        tmem_free(tm, TMEM_COLS);
+        tmem_free<PAIR>(tm, TMEM_COLS);
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------------------
@@ -999,8 +1035,9 @@ static Shape choose_shape(long long tilesM, long long N, int steps, int sms, con
             if (s > 1 && s > steps)
                 break;
             const long long waves = (tiles * s + sms - 1) / sms;
-            // split: every wave starts anew and ends with an exchange; otherwise tiles follow one another without a gap
-            const double cost = step * waves * ((steps + s - 1) / s) + (s > 1 ? waves * (5000.0 + 4.0 * bn) : 3000.0 + 4.0 * bn);
+            // split: every wave starts anew and ends with an exchange, and clusters of eight are slow to be placed (a 2048 x 2048
+            // product with one token: 10.3 us in eights, 5.9 in fours); otherwise tiles follow one another without a gap
+            const double cost = step * waves * ((steps + s - 1) / s) + (s > 1 ? waves * (5000.0 + 4.0 * bn) : 3000.0 + 4.0 * bn) + (s == 8 ? 9000.0 : 0.0);
             if (cost < bestCost)
             {
                 bestCost = cost;
@@ -1021,7 +1058,7 @@ static int smem_for(int stageBytes, int stages, int resultBytes)
 }
 
 template <class K, class... Args>
-static cudaError_t launch_cluster(K kernel, dim3 grid, int threads, int smem, int splits, cudaStream_t st, Args... args)
+static cudaError_t launch_cluster(K kernel, dim3 grid, int threads, int smem, dim3 cluster, cudaStream_t st, Args... args)
 {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess)
@@ -1033,9 +1070,9 @@ static cudaError_t launch_cluster(K kernel, dim3 grid, int threads, int smem, in
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = splits;
+    attr[0].val.clusterDim.x = cluster.x;
+    attr[0].val.clusterDim.y = cluster.y;
+    attr[0].val.clusterDim.z = cluster.z;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     e = cudaLaunchKernelEx(&cfg, kernel, args...);
@@ -1052,11 +1089,20 @@ template <bool WEIGHT, int FMT, int DENSE, class TD, class TO>
 static cudaError_t launch_grad(cudaStream_t st, const CUtensorMap& mc, const CUtensorMap& md, GradArgs a, int sms)
 {
     constexpr int NP = DENSE ? DENSE : 1;
-    const int stageBytes = a.bn * 128 * NP + grad_codes_bytes(FMT);
+    if constexpr (DENSE == 0)
+        if (a.bn == GRAD_PAIR)
+        {
+            const int stageBytes = GRAD_PAIR / 2 * 128 + grad_codes_bytes(FMT) + GRAD_SCALE_ROOM;
+            a.stages = stages_for(stageBytes, MAX_STAGES);
+            const auto kernel = k_mx_grad<WEIGHT, FMT, 0, true, TD, TO>;
+            const int smem = smem_for(stageBytes, a.stages, 0);
+            return launch_cluster(kernel, dim3((unsigned) (2 * std::min(a.tiles, sms / 2))), GradGroups<false, true>::threads, smem, dim3(2, 1, 1), st, mc, md, a);
+        }
+    const int stageBytes = a.bn * 128 * NP + grad_codes_bytes(FMT) + GRAD_SCALE_ROOM;
     a.stages = stages_for(stageBytes, MAX_STAGES);
     const int smem = smem_for(stageBytes, a.stages, a.splits > 1 ? 128 * (a.bn + 4) * 4 : 0);
     const dim3 grid((unsigned) (a.splits > 1 ? a.tiles : std::min(a.tiles, sms)), 1, (unsigned) a.splits);
-    return launch_cluster(k_mx_grad<WEIGHT, FMT, DENSE, TD, TO>, grid, GradGroups<(DENSE > 0)>::threads, smem, a.splits, st, mc, md, a);
+    return launch_cluster(k_mx_grad<WEIGHT, FMT, DENSE, false, TD, TO>, grid, GradGroups<(DENSE > 0), false>::threads, smem, dim3(1, 1, a.splits), st, mc, md, a);
 }
 
 template <bool WEIGHT, int FMT, class TO>
@@ -1067,6 +1113,16 @@ static cudaError_t launch_grad_dense(cudaStream_t st, const CUtensorMap& mc, con
     if (dyType == QAGG_F16)
         return launch_grad<WEIGHT, FMT, 2, __half, TO>(st, mc, md, a, sms);
     return launch_grad<WEIGHT, FMT, 3, float, TO>(st, mc, md, a, sms);
+}
+
+// Two CTAs on a 256 x 256 tile, or one on 128 x bn: cycles as in choose_shape, with what a pair waits for its one accumulator.
+static bool pair_pays(long long I, long long N, const GradArgs& a, int sms, int format)
+{
+    const int codes = grad_codes_bytes(format);
+    const double one = std::max(2.0 * a.bn, (codes + a.bn * 128.0) / 46.0) * ((a.tiles + sms - 1) / sms);
+    const long long pairs = (I + 255) / 256 * ((N + 255) / 256);
+    const double two = std::max(512.0, (codes + 16384.0) / 46.0) * 1.25 * ((pairs + sms / 2 - 1) / (sms / 2));
+    return two < one;
 }
 
 // What both gradients check and set up.  tokens x outputs is dy; `contraction` of the two is summed over.
@@ -1114,13 +1170,19 @@ static int grad_common(const char* who, bool weight, void* stream, const void* d
     a.splits = sh.splits;
     a.tilesM = (int) ((I + 127) / 128);
     a.tiles = a.tilesM * (int) ((N + a.bn - 1) / a.bn);
+    if (tma && a.splits == 1 && pair_pays(I, N, a, cfg.numSMs, format))
+    {
+        a.bn = GRAD_PAIR;
+        a.tilesM = (int) ((I + 255) / 256);
+        a.tiles = a.tilesM * (int) ((N + GRAD_PAIR - 1) / GRAD_PAIR);
+    }
     a.wide = weight ? ((((uintptr_t) out | (uintptr_t) (ldOut * 4)) & 15) == 0) : ((uintptr_t) out & 3) == 0 && (ldOut & 1) == 0;
     alignas(64) CUtensorMap mc, md;
     std::memset(&mc, 0, sizeof(mc));
     std::memset(&md, 0, sizeof(md));
     if (C > 0 && !codes_map(&mc, codes, I, C, format, format == QAGG_MXFP4 ? 64 : 128, GK))
         return fail(QAGG_ECUDA, std::string(who) + ": tensor map of the codes could not be made");
-    if (C > 0 && tma && !encode_map_tiled(&md, 2, dy, O, T, ldDy * 2, 64, weight ? GK : a.bn, 128))
+    if (C > 0 && tma && !encode_map_tiled(&md, 2, dy, O, T, ldDy * 2, 64, weight ? GK : a.bn == GRAD_PAIR ? GRAD_PAIR / 2 : a.bn, 128))
         return fail(QAGG_ECUDA, std::string(who) + ": tensor map of dy could not be made");
     const cudaStream_t st = (cudaStream_t) stream;
     cudaError_t e;
@@ -1197,12 +1259,15 @@ int qagg_mx_times(void* stream, const void* w_codes, const void* w_scales, const
     const dim3 grid((unsigned) (a.splits > 1 ? a.tiles : std::min(a.tiles, cfg.numSMs)), 1, (unsigned) a.splits);
     const cudaStream_t st = (cudaStream_t) stream;
     cudaError_t e;
+    const dim3 cluster(1, 1, a.splits);
+    const bool narrow = a.bn <= TIMES_NARROW;
     if (y_type == QAGG_F32)
-        e = launch_cluster(k_mx_times<float>, grid, TT, smem, a.splits, st, mw, mx, a);
+        e = narrow ? launch_cluster(k_mx_times<float, TIMES_NARROW>, grid, TT, smem, cluster, st, mw, mx, a) : launch_cluster(k_mx_times<float, 128>, grid, TT, smem, cluster, st, mw, mx, a);
     else if (y_type == QAGG_F16)
-        e = launch_cluster(k_mx_times<__half>, grid, TT, smem, a.splits, st, mw, mx, a);
+        e = narrow ? launch_cluster(k_mx_times<__half, TIMES_NARROW>, grid, TT, smem, cluster, st, mw, mx, a) : launch_cluster(k_mx_times<__half, 128>, grid, TT, smem, cluster, st, mw, mx, a);
     else
-        e = launch_cluster(k_mx_times<__nv_bfloat16>, grid, TT, smem, a.splits, st, mw, mx, a);
+        e = narrow ? launch_cluster(k_mx_times<__nv_bfloat16, TIMES_NARROW>, grid, TT, smem, cluster, st, mw, mx, a)
+                   : launch_cluster(k_mx_times<__nv_bfloat16, 128>, grid, TT, smem, cluster, st, mw, mx, a);
     return check_cuda(e, "4-bit product kernel launch");
 }
 

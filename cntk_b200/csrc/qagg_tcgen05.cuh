@@ -28,6 +28,15 @@ __device__ __forceinline__ bool mbar_suspend_wait(unsigned long long* bar, unsig
                  : "memory");
     return ok != 0;
 }
+// Arrive at the same barrier of CTA `rank` of the cluster.  CTA scope is enough here, and a release to the whole cluster cost the warp
+// 1900 cycles each time: what the arrival announces is this SM's own tensor and shared memory, and it is this SM's half of the
+// pair's product that reads them.
+__device__ __forceinline__ void mbar_arrive_remote(unsigned long long* bar, unsigned rank)
+{
+    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, %1;\n\tmbarrier.arrive.shared::cluster.b64 _, [r];\n\t}" ::"r"(smem_addr(bar)),
+                 "r"(rank)
+                 : "memory");
+}
 __device__ __forceinline__ void tc_wait(unsigned long long* bar, unsigned parity, unsigned* broken, unsigned* status)
 {
     if (mbar_suspend_wait(bar, parity))
@@ -76,13 +85,27 @@ __device__ __forceinline__ void fence_async_shared()
 
 // ---- tensor memory ------------------------------------------------------------------------------------------------------------
 // 128 lanes x 512 columns of 32 bits; warp w of a CTA reaches lanes 32 * (w % 4) .. + 31.  An address is lane << 16 | column.
+// PAIR: for products that two CTAs of a cluster (ranks 0 and 1) make together; both of them call these.
+template <bool PAIR = false>
 __device__ __forceinline__ void tmem_alloc(unsigned* slot, unsigned columns)
 {
+    if constexpr (PAIR)
+    {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(slot)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        return;
+    }
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(slot)), "r"(columns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
 }
+template <bool PAIR = false>
 __device__ __forceinline__ void tmem_free(unsigned base, unsigned columns)
 {
+    if constexpr (PAIR)
+    {
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns));
+        return;
+    }
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns));
 }
 __device__ __forceinline__ void tc_fence_before()
@@ -151,10 +174,10 @@ __device__ __forceinline__ unsigned long long smem_desc(unsigned addr, unsigned 
     return (unsigned long long) ((addr >> 4) & 0x3fffu) | ((unsigned long long) ((leading >> 4) & 0x3fffu) << 16) |
            ((unsigned long long) ((stride >> 4) & 0x3fffu) << 32) | (1ull << 46) | ((unsigned long long) swizzle << 61);
 }
-// bf16 x bf16 -> fp32, 128 x n; transB: operand B is MN-major
-__host__ __device__ constexpr unsigned idesc_bf16(int n, bool transB)
+// bf16 x bf16 -> fp32, m x n; transB: operand B is MN-major
+__host__ __device__ constexpr unsigned idesc_bf16(int n, bool transB, int m = 128)
 {
-    return (1u << 4) | (1u << 7) | (1u << 10) | ((transB ? 1u : 0u) << 16) | ((unsigned) (n >> 3) << 17) | ((128u >> 4) << 24);
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((transB ? 1u : 0u) << 16) | ((unsigned) (n >> 3) << 17) | ((unsigned) (m >> 4) << 24);
 }
 // e2m1 x e2m1 with one power-of-two scale per 32 values -> fp32, 128 x n; sf: which pair of a scale word's four bytes
 __host__ __device__ constexpr unsigned idesc_mxf4(int n, unsigned sf)
@@ -166,6 +189,14 @@ __device__ __forceinline__ void mma_bf16_ts(unsigned d, unsigned a, unsigned lon
 {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((unsigned) add)
+                 : "memory");
+}
+// The same by two CTAs: 256 rows, 128 of A and D in each one's tensor memory, half of B's columns in each one's shared memory, at the same
+// addresses.  Issued by rank 0.
+__device__ __forceinline__ void mma_bf16_ts_pair(unsigned d, unsigned a, unsigned long long b, unsigned idesc, bool add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((unsigned) add)
                  : "memory");
 }
 // D (+)= A B over 64 contraction values, both in shared memory, block scales in tensor memory
@@ -180,6 +211,13 @@ __device__ __forceinline__ void mma_mxf4_ss(unsigned d, unsigned long long a, un
 __device__ __forceinline__ void tc_commit(unsigned long long* bar)
 {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+// the same for products of two CTAs: arrives at the barrier of both
+__device__ __forceinline__ void tc_commit_pair(unsigned long long* bar)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(bar)), "h"((unsigned short) 3)
+                 : "memory");
 }
 
 // ---- clusters -----------------------------------------------------------------------------------------------------------------
