@@ -146,6 +146,38 @@ __device__ __forceinline__ void take_chain(GemmBars* bars, int buf, unsigned par
             mbar_arrive(&bars->taken[buf]);
     }
 }
+// A CTA's only tile with a single chain goes from tensor memory to its place sixteen columns at a time: the loop is a tenth of the code that
+// registers holding the whole tile need, and a launch of a few microseconds spends much of them on fetching instructions.
+// f(j, values): columns j .. j + 15.
+template <class F>
+__device__ __forceinline__ void drain_chain(GemmBars* bars, unsigned tmem, int cols, bool nothing, F f)
+{
+    if (!nothing)
+        tc_wait(&bars->ready[0], 0, &bars->broken, &g_mxStatus);
+    __syncwarp();
+    tc_fence_after();
+#pragma unroll 1
+    for (int j = 0; j < cols; j += 16)
+    {
+        float v[16];
+        if (nothing)
+        {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                v[e] = 0.0f;
+        }
+        else
+        {
+            unsigned r[16];
+            tmem_load16(tmem + j, r);
+            tmem_load_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                v[e] = __uint_as_float(r[e]);
+        }
+        f(j, v);
+    }
+}
 // Which accumulator a chain uses, and the parity of its barriers' phase.
 struct Chains
 {
@@ -236,45 +268,71 @@ __device__ __forceinline__ void write_row(float* out, long long ld, long long m,
 
 // Split contraction: each CTA leaves its partial sums in its shared memory ([n][128 rows], or for rows [m][bn + 4]), and CTA `rank` adds
 // up and writes its share of the tile's columns (rows).  Called by all threads; result warps have put their sums down.
-template <bool ROWS, class T>
-__device__ __forceinline__ void reduce_cluster(float* buf, int splits, int rank, int bn, T* out, long long ld, long long m0, long long M, long long n0, long long N,
-                                               const float* bias, bool add)
+// wide: four neighbours of the output are one aligned word of 4 * sizeof(T) bytes.
+__device__ __forceinline__ void put4(float* p, const float4& s) { *reinterpret_cast<float4*>(p) = s; }
+template <class T>
+__device__ __forceinline__ void put4(T* p, const float4& s)
 {
-    __syncwarp();
-    cluster_sync();
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack2(s.x, s.y, p), pack2(s.z, s.w, p));
+}
+template <int SPLITS, bool ROWS, class T>
+__device__ __forceinline__ void reduce_parts(float* buf, int rank, int bn, T* out, long long ld, long long m0, long long M, long long n0, long long N, const float* bias,
+                                             bool add, bool wide)
+{
     const long long restM = M - m0, restN = N - n0;
     const int rows = (int) (restM < 128 ? restM : 128), cols = (int) (restN < bn ? restN : bn);
     const int pitch = ROWS ? bn + 4 : 128;
     const int lines = ROWS ? rows : cols, width = ROWS ? cols : rows;
     const int perLine = (width + 3) / 4;
-    const int u1 = (int) ((long long) lines * perLine * (rank + 1) / splits);
-    for (int u = (int) ((long long) lines * perLine * rank / splits) + (int) threadIdx.x; u < u1; u += blockDim.x)
+    const int u1 = lines * perLine * (rank + 1) / SPLITS;
+#pragma unroll 1
+    for (int u = lines * perLine * rank / SPLITS + (int) threadIdx.x; u < u1; u += blockDim.x)
     {
         const int l = u / perLine, w = (u - l * perLine) * 4;
         const unsigned at = smem_addr(buf + l * pitch + w);
-        float4 v[8];
+        float4 v[SPLITS];
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (k < splits)
-                v[k] = cluster_load4(cluster_address(at, k));
-        float4 s = v[0];
-#pragma unroll
-        for (int k = 1; k < 8; ++k)
-            if (k < splits)
-                s = make_float4(s.x + v[k].x, s.y + v[k].y, s.z + v[k].z, s.w + v[k].w);
-        const float e[4] = {s.x, s.y, s.z, s.w};
+        for (int k = 0; k < SPLITS; ++k)
+            v[k] = cluster_load4(cluster_address(at, k));
         const long long col = (ROWS ? n0 : m0) + w;
         T* p = out + ((ROWS ? m0 : n0) + l) * ld + col;
+        float4 s = v[0];
+#pragma unroll
+        for (int k = 1; k < SPLITS; ++k)
+            s = make_float4(s.x + v[k].x, s.y + v[k].y, s.z + v[k].z, s.w + v[k].w);
+        float e[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (w + j < width)
             {
                 if constexpr (ROWS)
-                    p[j] = add ? p[j] + e[j] : e[j];
+                    e[j] += add ? (float) p[j] : 0.0f;
                 else
-                    put(p + j, e[j] + (bias ? bias[col + j] : 0.0f));
+                    e[j] += bias ? bias[col + j] : 0.0f;
             }
+        if (wide && w + 4 <= width)
+            put4(p, make_float4(e[0], e[1], e[2], e[3]));
+        else
+        {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (w + j < width)
+                    put(p + j, e[j]);
+        }
     }
+}
+template <bool ROWS, class T>
+__device__ __forceinline__ void reduce_cluster(float* buf, int splits, int rank, int bn, T* out, long long ld, long long m0, long long M, long long n0, long long N,
+                                               const float* bias, bool add, bool wide)
+{
+    __syncwarp();
+    cluster_sync();
+    if (splits == 2)
+        reduce_parts<2, ROWS>(buf, rank, bn, out, ld, m0, M, n0, N, bias, add, wide);
+    else if (splits == 4)
+        reduce_parts<4, ROWS>(buf, rank, bn, out, ld, m0, M, n0, N, bias, add, wide);
+    else
+        reduce_parts<8, ROWS>(buf, rank, bn, out, ld, m0, M, n0, N, bias, add, wide);
     __syncwarp();
     cluster_sync(); // nobody leaves while its partial sums are being read
 }
@@ -306,7 +364,8 @@ struct TimesArgs
     const float* bias;
     void* y;
     long long ld, O, T, K;
-    int bn, stages, splits, tilesM, tiles, pairs;
+    int bn, stages, splits, tilesM, tiles;
+    int pairs, wide4; // y: two rows of a column can be written at once, four of them
 };
 
 constexpr int TT = 384;  // copy, product, allocating and spare warp; eight result warps
@@ -479,15 +538,26 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
             for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
             {
                 const long long m0 = (long long) (tile % a.tilesM) * 128, n0 = (long long) (tile / a.tilesM) * bn;
+                const float bias = a.bias && a.splits == 1 && m0 + m < a.O ? a.bias[m0 + m] : 0.0f;
+                float* buf = reinterpret_cast<float*>(stage0);
+                if (a.tiles <= (int) gridDim.x && count <= CHAIN_STEPS)
+                {
+                    drain_chain(&bars, mine, cols, count == 0, [&](int j, const float(&v)[16]) {
+                        if (a.splits > 1)
+                            put_partial<false>(buf, bn, m, half * 128 + j, 16, v);
+                        else
+                            write_columns((T*) a.y, a.ld, m0 + m, a.O, n0 + half * 128 + j, a.T, 16, v, bias, lane ^ 1, a.pairs && m0 + 128 <= a.O);
+                    });
+                    break;
+                }
                 float acc[ACC];
 #pragma unroll
                 for (int j = 0; j < ACC; ++j)
                     acc[j] = 0.0f;
-                const float bias = a.bias && a.splits == 1 && m0 + m < a.O ? a.bias[m0 + m] : 0.0f;
                 for (int i = 0; i < count; i += CHAIN_STEPS, chain.next(bufs))
                     take_chain<false>(&bars, chain.buf, chain.par, mine + chain.buf * 128, cols, i == 0, acc);
                 if (a.splits > 1)
-                    put_partial<false>(reinterpret_cast<float*>(stage0), bn, m, half * 128, cols, acc);
+                    put_partial<false>(buf, bn, m, half * 128, cols, acc);
                 else
                     write_columns((T*) a.y, a.ld, m0 + m, a.O, n0 + half * 128, a.T, cols, acc, bias, lane ^ 1, a.pairs && m0 + 128 <= a.O);
             }
@@ -496,7 +566,7 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
     __syncwarp();
     if (a.splits > 1) // one tile per cluster
         reduce_cluster<false, T>(reinterpret_cast<float*>(stage0), a.splits, rank, bn, (T*) a.y, a.ld, (long long) (blockIdx.x % a.tilesM) * 128, a.O,
-                                 (long long) (blockIdx.x / a.tilesM) * bn, a.T, a.bias, false);
+                                 (long long) (blockIdx.x / a.tilesM) * bn, a.T, a.bias, false, a.wide4);
     tc_fence_before();
     __syncthreads();
     if (warp == 2)
@@ -517,7 +587,7 @@ struct GradArgs
     long long N;        // the other dimension
     int bn, stages, splits, tilesM, tiles;
     int vec;            // dy can be read 16 bytes a time
-    int wide;           // out: rows can be written 16 bytes a time, columns in pairs of rows
+    int wide, wide4;    // out: rows can be written 16 bytes a time, columns in pairs of rows; four neighbours at once
     int add;
 };
 
@@ -701,6 +771,59 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
         }
         early = count < S ? count : S;
         __syncwarp();
+    }
+    // Loaders of the dense operand: rows of 64 contiguous values (128 bytes a plane), in units of eight values, two a thread and step.
+    constexpr int THREADS = DENSE ? 128 * G::load : 1024, UNITS = 1024 / THREADS; // bn <= 128: at most 1024 units
+    struct Units
+    {
+        Raw8<TD> raw[UNITS];
+    };
+    const TD* dy = (const TD*) a.dy;
+    const int t = threadIdx.x - G::firstLoad * 32;
+    const long long stepStride = WEIGHT ? GK * a.ldDy : GK;
+    const TD* from[UNITS]; // the unit's next values
+    int have[UNITS];       // WEIGHT: how many of its eight columns exist; otherwise whether its token does
+    int left = 0;          // contraction values from the next step on
+    int nextTile = firstTile, nextStep = 0;
+    auto fetch = [&](Units& v) { // the next step that this CTA has
+        if (nextTile >= a.tiles || count == 0)
+            return;
+        if (nextStep == 0)
+        {
+            const long long n0 = tile_n0(nextTile), k0 = (long long) first * GK;
+            left = (int) (a.C - k0);
+#pragma unroll
+            for (int q = 0; q < UNITS; ++q)
+            {
+                const int u = t + q * THREADS;
+                const int c = u & 7, r = WEIGHT ? (u >> 3) & 63 : u >> 3, atom = WEIGHT ? u >> 9 : 0;
+                const long long col = (WEIGHT ? n0 + atom * 64 : k0) + c * 8, line = (WEIGHT ? k0 : n0) + r; // output, token
+                const long long cols = a.N - col;
+                from[q] = dy + line * a.ldDy + col;
+                have[q] = u >= bn * 8 ? 0 : WEIGHT ? (cols < 0 ? 0 : cols < 8 ? (int) cols : 8) : line < a.N;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < UNITS; ++q)
+        {
+            const int u = t + q * THREADS;
+            const int rest = left - (WEIGHT ? (u >> 3) & 63 : (u & 7) * 8);
+            const int n = WEIGHT ? (rest > 0 ? have[q] : 0) : (have[q] ? min(max(rest, 0), 8) : 0);
+            v.raw[q] = load8(from[q], n, a.vec);
+            from[q] += stepStride;
+        }
+        left -= GK;
+        if (++nextStep == count)
+        {
+            nextStep = 0;
+            nextTile += tileStep;
+        }
+    };
+    Units even = {}, odd = {};
+    if (DENSE > 0 && warp >= G::firstLoad)
+    {
+        fetch(even);
+        fetch(odd);
     }
     if (warp == 2)
         tmem_alloc<PAIR>(&bars.tmem, TMEM_COLS);
@@ -903,6 +1026,20 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
             for (int tile = firstTile; tile < a.tiles; tile += tileStep)
             {
                 const long long m0 = tile_m0(tile), n0 = tile_n0(tile);
+                float* buf = reinterpret_cast<float*>(stage0);
+                const int partner = lane ^ (FMT == QAGG_MXFP4 ? 8 : 1);
+                if (!PAIR && a.tiles <= tileStep && count <= CHAIN_STEPS)
+                {
+                    drain_chain(&bars, mine, cols, count == 0, [&](int j, const float(&v)[16]) {
+                        if (a.splits > 1)
+                            put_partial<WEIGHT>(buf, bn, m, half * cols + j, 16, v);
+                        else if constexpr (WEIGHT)
+                            write_row((float*) a.out, a.ld, m0 + m, a.I, n0 + half * cols + j, a.N, 16, v, a.add != 0, a.wide != 0);
+                        else
+                            write_columns((TO*) a.out, a.ld, m0 + m, a.I, n0 + half * cols + j, a.N, 16, v, 0.0f, partner, a.wide && m0 + 128 <= a.I);
+                    });
+                    break;
+                }
                 constexpr int ACC = WIDEST / G::result;
                 float acc[ACC];
 #pragma unroll
@@ -911,50 +1048,21 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
                 for (int i = 0; i < count; i += CHAIN_STEPS, chain.next(BUFS))
                     take_chain<PAIR>(&bars, chain.buf, chain.par, mine + chain.buf * WIDEST, cols, i == 0, acc);
                 if (!PAIR && a.splits > 1)
-                    put_partial<WEIGHT>(reinterpret_cast<float*>(stage0), bn, m, half * cols, cols, acc);
+                    put_partial<WEIGHT>(buf, bn, m, half * cols, cols, acc);
                 else if constexpr (WEIGHT)
                     write_row((float*) a.out, a.ld, m0 + m, a.I, n0 + half * cols, a.N, cols, acc, a.add != 0, a.wide != 0);
                 else
-                    write_columns((TO*) a.out, a.ld, m0 + m, a.I, n0 + half * cols, a.N, cols, acc, 0.0f, lane ^ (FMT == QAGG_MXFP4 ? 8 : 1), a.wide && m0 + 128 <= a.I);
+                    write_columns((TO*) a.out, a.ld, m0 + m, a.I, n0 + half * cols, a.N, cols, acc, 0.0f, partner, a.wide && m0 + 128 <= a.I);
             }
         }
     }
-    else
+    else if constexpr (DENSE > 0)
     {
-        // Bring the dense operand: rows of 64 contiguous values (128 bytes a plane), eight values a thread and turn.  Two steps' values
-        // are on their way (behind the fence, which would wait for them) while an earlier one is split and stored.
+        // Two steps' values are on their way (behind the fence, which would wait for them) while an earlier one is split and stored.
         registers_down<G::regsLoad>();
-        const TD* dy = (const TD*) a.dy;
-        const int t = threadIdx.x - G::firstLoad * 32;
-        constexpr int UNITS = 2; // bn <= 128: at most 1024 pieces for 512 threads
-        struct Step
-        {
-            Raw8<TD> raw[UNITS];
-        };
-        int nextTile = firstTile, nextStep = 0;
-        auto fetch = [&](Step& st) { // the next step that this CTA has
-            if (nextTile >= a.tiles || count == 0)
-                return;
-            const long long n0 = tile_n0(nextTile), k0 = (long long) (first + nextStep) * GK;
-#pragma unroll
-            for (int q = 0; q < UNITS; ++q)
-            {
-                const int u = t + q * 512;
-                const int c = u & 7, r = WEIGHT ? (u >> 3) & 63 : u >> 3, atom = WEIGHT ? u >> 9 : 0;
-                const long long line = WEIGHT ? k0 + r : n0 + r;              // token
-                const long long col = (WEIGHT ? n0 + atom * 64 : k0) + c * 8; // output
-                const long long left = (WEIGHT ? a.N : a.C) - col;
-                st.raw[q] = load8(dy + line * a.ldDy + col, u < bn * 8 && line < (WEIGHT ? a.C : a.N) ? (left < 0 ? 0 : left < 8 ? (int) left : 8) : 0, a.vec);
-            }
-            if (++nextStep == count)
-            {
-                nextStep = 0;
-                nextTile += tileStep;
-            }
-        };
         Ring ring;
         long long done = 0;
-        auto put_step = [&](Step& st) {
+        auto put_step = [&](const Units& v) {
             if (done >= S)
                 tc_wait(&bars.empty[ring.s], ring.par ^ 1, &bars.broken, &g_mxStatus);
             ++done;
@@ -962,16 +1070,16 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
 #pragma unroll
             for (int q = 0; q < UNITS; ++q)
             {
-                const int u = t + q * 512;
+                const int u = t + q * THREADS;
                 const int c = u & 7, r = WEIGHT ? (u >> 3) & 63 : u >> 3, atom = WEIGHT ? u >> 9 : 0;
                 unsigned char* dst = at + atom * 8192 + r * 128 + ((c ^ (r & 7)) << 4);
                 unsigned w[NP][4];
                 if (NP == 1)
-                    *reinterpret_cast<uint4*>(w[0]) = st.raw[q].a;
-                else if (any_special(st.raw[q]))
-                    split8<TD, NP, true>(st.raw[q], w);
+                    *reinterpret_cast<uint4*>(w[0]) = v.raw[q].a;
+                else if (any_special(v.raw[q]))
+                    split8<TD, NP, true>(v.raw[q], w);
                 else
-                    split8<TD, NP, false>(st.raw[q], w);
+                    split8<TD, NP, false>(v.raw[q], w);
 #pragma unroll
                 for (int p = 0; p < NP; ++p)
                     if (u < bn * 8)
@@ -983,9 +1091,6 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
                 mbar_arrive(&bars.dense[ring.s]);
             ring.next(S);
         };
-        Step even, odd;
-        fetch(even);
-        fetch(odd);
         const long long mySteps = firstTile < a.tiles ? (long long) ((a.tiles - 1 - firstTile) / tileStep + 1) * count : 0;
         for (long long n = 0; n < mySteps; n += 2)
         {
@@ -1001,7 +1106,7 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
     __syncwarp();
     if (!PAIR && a.splits > 1) // one tile per cluster
         reduce_cluster<WEIGHT, TO>(reinterpret_cast<float*>(stage0), a.splits, rank, bn, (TO*) a.out, a.ld, tile_m0(blockIdx.x), a.I, tile_n0(blockIdx.x), a.N, nullptr,
-                                   a.add != 0);
+                                   a.add != 0, a.wide4);
     tc_fence_before();
     if (PAIR)
         cluster_sync(); // neither goes while the other may still arrive at its barriers or use its memory
@@ -1177,6 +1282,7 @@ static int grad_common(const char* who, bool weight, void* stream, const void* d
         a.tiles = a.tilesM * (int) ((N + GRAD_PAIR - 1) / GRAD_PAIR);
     }
     a.wide = weight ? ((((uintptr_t) out | (uintptr_t) (ldOut * 4)) & 15) == 0) : ((uintptr_t) out & 3) == 0 && (ldOut & 1) == 0;
+    a.wide4 = (((uintptr_t) out | (uintptr_t) (ldOut * mx_type_bytes(outType))) & (4 * mx_type_bytes(outType) - 1)) == 0;
     alignas(64) CUtensorMap mc, md;
     std::memset(&mc, 0, sizeof(mc));
     std::memset(&md, 0, sizeof(md));
@@ -1248,6 +1354,7 @@ int qagg_mx_times(void* stream, const void* w_codes, const void* w_scales, const
     a.tilesM = (int) ((O + 127) / 128);
     a.tiles = a.tilesM * (int) ((T + a.bn - 1) / a.bn);
     a.pairs = ((uintptr_t) y & 3) == 0 && (ld_y & 1) == 0;
+    a.wide4 = (((uintptr_t) y | (uintptr_t) (ld_y * mx_type_bytes(y_type))) & (4 * mx_type_bytes(y_type) - 1)) == 0;
     const int stageBytes = times_stage_bytes(a.bn);
     a.stages = stages_for(stageBytes, MAX_STAGES);
     const int smem = smem_for(stageBytes, a.stages, a.splits > 1 ? 128 * a.bn * 4 : 0);
