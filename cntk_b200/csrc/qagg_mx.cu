@@ -2,21 +2,28 @@
 // that keep their input in 8 bits for the backward pass.  The form is described in qagg_mx.cuh.
 //
 // All kernels here move each value once and are bound by HBM.  One CTA takes one scale tile: 128 packed columns x 4 blocks.
-// Sixteen threads share a column's 128 rows, eight values each (one 16-byte load of a 16-bit type), so a block's largest magnitude
-// takes two shuffles and the tile's 512 scale bytes are collected in shared memory and leave as full lines.
+// A thread takes 16 bytes of dense values at a time (eight of a 16-bit type, four fp32: whole warps then read and write whole lines),
+// so four or eight threads share a block, its largest magnitude takes two or three shuffles, and the tile's 512 scale bytes are
+// collected in shared memory and leave as full lines.
 #include "qagg_mx.cuh"
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 namespace qagg {
 
-constexpr int MXT = 256;              // threads per CTA
-constexpr int MX_TILE = 128;          // rows and columns of a tile
-constexpr int MX_PASS = MXT / 16;     // columns per pass
-constexpr int MX_PASSES = MX_TILE / MX_PASS;
-
-// ---- eight values of one column -------------------------------------------------------------------------------------------
+constexpr int MXT = 256;     // threads per CTA
+constexpr int MX_TILE = 128; // rows and columns of a tile
+template <class T, bool ACT = false>
+struct Shape // of the threads over a tile; ACT: with a function's arithmetic, which needs the registers
+{
+    static constexpr int V = 16 / sizeof(T);             // values per thread and turn
+    static constexpr int LANES = MX_TILE / V;            // threads per column
+    static constexpr int COLS = MXT / LANES;             // columns per pass
+    static constexpr int PASSES = MX_TILE / COLS;
+    static constexpr int FLIGHT = ACT ? 4 : 8; // passes whose loads are in flight together
+};
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
@@ -30,33 +37,44 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// 16 bytes of values: n of them exist, the others read as zero.  vec: the address is 16-byte aligned.
 template <class T>
-__device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&v)[8])
+__device__ __forceinline__ uint4 load16(const T* p, int n, bool vec)
+{
+    constexpr int V = Shape<T>::V;
+    uint4 r = make_uint4(0, 0, 0, 0);
+    if (vec && n == V)
+        return __ldcs(reinterpret_cast<const uint4*>(p));
+    T* e = reinterpret_cast<T*>(&r);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (i < n)
+            e[i] = p[i];
+    return r;
+}
+template <class T>
+__device__ __forceinline__ void unpack16(const uint4& r, float (&v)[Shape<T>::V])
 {
     const T* e = reinterpret_cast<const T*>(&r);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < Shape<T>::V; ++i)
         v[i] = to_float(e[i]);
 }
 template <class T>
-__device__ __forceinline__ void store8(T* p, const float (&v)[8], int n, bool vec)
+__device__ __forceinline__ void store16(T* p, const float (&v)[Shape<T>::V], int n, bool vec)
 {
-    Raw8<T> r;
+    constexpr int V = Shape<T>::V;
+    uint4 r;
     T* e = reinterpret_cast<T*>(&r);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < V; ++i)
         e[i] = from_float<T>(v[i]);
-    if (vec && n == 8)
-    {
-        uint4* q = reinterpret_cast<uint4*>(p);
-        __stcs(q, r.a);
-        if constexpr (sizeof(T) == 4)
-            __stcs(q + 1, r.b);
-    }
+    if (vec && n == V)
+        __stcs(reinterpret_cast<uint4*>(p), r);
     else
     {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < V; ++i)
             if (i < n)
                 p[i] = e[i];
     }
@@ -77,169 +95,231 @@ __device__ __forceinline__ unsigned scale_byte(unsigned top)
 
 // x / 2^X is exact (a value whose quotient is subnormal is far below the first rounding border).  int8: q by adding 1.5 * 2^23,
 // which rounds to an integer, ties to even, in the low bits.  fp4: the hardware's conversion, nearest even, held at 6.
-template <int FMT, int N>
-__device__ __forceinline__ void encode(const float (&v)[N], unsigned byte, unsigned (&out)[N / (FMT == QAGG_MXFP4 ? 8 : 4)])
+template <int FMT>
+__device__ __forceinline__ unsigned encode4(float a, float b, float c, float d, float inv) // four int8 or (in 16 bits) four fp4 codes
 {
-    const float inv = mx_scale_inv(byte);
-    const bool bad = byte == 255u;
     if constexpr (FMT == QAGG_MXFP4)
-    {
-#pragma unroll
-        for (int w = 0; w < N / 8; ++w)
-        {
-            unsigned r = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                r |= (unsigned) __nv_cvt_float2_to_fp4x2(make_float2(v[8 * w + 2 * i] * inv, v[8 * w + 2 * i + 1] * inv), __NV_E2M1, cudaRoundNearest) << (8 * i);
-            out[w] = bad ? 0u : r;
-        }
-    }
+        return (unsigned) __nv_cvt_float2_to_fp4x2(make_float2(a * inv, b * inv), __NV_E2M1, cudaRoundNearest) |
+               (unsigned) __nv_cvt_float2_to_fp4x2(make_float2(c * inv, d * inv), __NV_E2M1, cudaRoundNearest) << 8;
     else
     {
-#pragma unroll
-        for (int w = 0; w < N / 4; ++w)
-        {
-            unsigned q[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-            {
-                const float a = fminf(fmaxf(v[4 * w + i] * inv, -127.0f / 64.0f), 127.0f / 64.0f);
-                q[i] = __float_as_uint(__fmaf_rn(a, 64.0f, 12582912.0f));
-            }
-            const unsigned r = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
-            out[w] = bad ? 0u : r;
-        }
-    }
-}
-// eight elements -> values
-template <int FMT>
-__device__ __forceinline__ void decode8(const unsigned* w, unsigned byte, float (&v)[8])
-{
-    const float s = byte == 255u ? __uint_as_float(0x7fffffffu) : mx_scale(byte);
-    if constexpr (FMT == QAGG_MXFP4)
-    {
+        const float v[4] = {a, b, c, d};
+        unsigned q[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-        {
-            const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t) (w[0] >> (8 * i)), __NV_E2M1);
-            const float2 f = __half22float2(__half2(h));
-            v[2 * i] = f.x * s;
-            v[2 * i + 1] = f.y * s;
-        }
+            q[i] = __float_as_uint(__fmaf_rn(fminf(fmaxf(v[i] * inv, -127.0f / 64.0f), 127.0f / 64.0f), 64.0f, 12582912.0f));
+        return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+    }
+}
+// four codes -> values; s: the block's scale, NaN for a bad block
+template <int FMT>
+__device__ __forceinline__ void decode4(unsigned w, float s, float& a, float& b, float& c, float& d)
+{
+    if constexpr (FMT == QAGG_MXFP4)
+    {
+        const float2 lo = __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t) (w & 0xffu), __NV_E2M1)));
+        const float2 hi = __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t) (w >> 8 & 0xffu), __NV_E2M1)));
+        a = lo.x * s, b = lo.y * s, c = hi.x * s, d = hi.y * s;
     }
     else
     {
-        // element first, then the scale: q / 64 * 2^X, each product exact, down to the smallest scale
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = ((float) (signed char) (w[i / 4] >> (8 * (i % 4))) * 0.015625f) * s;
+        // q by way of 2^23 + 128 + q (an integer in the low bits); element first, then the scale: q / 64 * 2^X, each product exact, down
+        // to the smallest scale
+        const unsigned u = w ^ 0x80808080u;
+        a = __fmaf_rn(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)), 0.015625f, -131074.0f) * s;
+        b = __fmaf_rn(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441)), 0.015625f, -131074.0f) * s;
+        c = __fmaf_rn(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)), 0.015625f, -131074.0f) * s;
+        d = __fmaf_rn(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443)), 0.015625f, -131074.0f) * s;
     }
+}
+__device__ __forceinline__ float block_scale(unsigned byte)
+{
+    return byte == 255u ? __uint_as_float(0x7fffffffu) : mx_scale(byte);
 }
 
 // ---- pointwise functions -----------------------------------------------------------------------------------------------------
+// In fp32 whatever the type, within about 1e-7 * (1 + |x|): with the hardware's exponential and reciprocal, whose errors of a few
+// units of 2^-23 apply to e = exp(-|x|) <= 1, so that no form here overflows or cancels.  With expf, erff and IEEE divisions the
+// kernels were bound by their instructions: gelu of 4096 x 8192 bf16 took 53 us forward and 66 backward for 26 us of HBM traffic each.
+__device__ __forceinline__ float exp2_approx(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp_approx(float x)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// exp(-k |x|)
+__device__ __forceinline__ float exp_minus(float k, float x)
+{
+    return exp2_approx(fabsf(x) * (-1.4426950408889634f * k));
+}
 
-template <int ACT>
+// Phi(-|x|), the normal distribution's lower tail, and e = exp(-x^2 / 2): erfc(z) = (a1 t + ... + a5 t^5) exp(-z^2), t = 1 / (1 + p z), off by at
+// most 1.5e-7 (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26), at z = |x| / sqrt(2); its half.
+__device__ __forceinline__ float normal_tail(float x, float& e)
+{
+    const float t = rcp_approx(__fmaf_rn(0.3275911f * 0.70710678118654752f, fabsf(x), 1.0f));
+    e = exp2_approx(x * x * (-0.5f * 1.4426950408889634f));
+    float p = __fmaf_rn(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+    p = __fmaf_rn(p, t, 0.5f * 1.421413741f);
+    p = __fmaf_rn(p, t, 0.5f * -0.284496736f);
+    p = __fmaf_rn(p, t, 0.5f * 0.254829592f);
+    return p * t * e;
+}
+
+template <int ACT, class T>
 __device__ __forceinline__ float act_value(float x)
 {
     if constexpr (ACT == QAGG_ACT_RELU)
         return x > 0.0f ? x : (x != x ? x : 0.0f);
-    else if constexpr (ACT == QAGG_ACT_SIGMOID)
-        return __fdiv_rn(1.0f, 1.0f + expf(-x));
     else if constexpr (ACT == QAGG_ACT_TANH)
-        return tanhf(x);
+    {
+        if constexpr (sizeof(T) == 4)
+            return tanhf(x); // relative precision near 0
+        else
+        {
+            const float e = exp_minus(2.0f, x);
+            const float t = (1.0f - e) * rcp_approx(1.0f + e);
+            return fabsf(x) < 0.02f ? __fmaf_rn(x * x * x, -0.33333333f, x) : copysignf(t, x);
+        }
+    }
     else if constexpr (ACT == QAGG_ACT_GELU)
-        return x * (0.5f * (1.0f + erff(x * 0.70710678118654752f)));
+    {
+        float e;
+        const float tail = normal_tail(x, e);
+        return __fmaf_rn(-fabsf(x), tail, x > 0.0f ? x : x * 0.0f); // x - x tail or x tail; NaN stays
+    }
     else
-        return __fdiv_rn(x, 1.0f + expf(-x));
+    {
+        const float e = exp_minus(1.0f, x), r = rcp_approx(1.0f + e);
+        const float s = x < 0.0f ? e * r : r; // the sigmoid of x
+        return ACT == QAGG_ACT_SIGMOID ? s : x * s;
+    }
 }
-// derivative; with e = exp(-|x|) no form here overflows or cancels
+// derivative
 template <int ACT>
 __device__ __forceinline__ float act_slope(float x)
 {
     if constexpr (ACT == QAGG_ACT_RELU)
         return x > 0.0f ? 1.0f : (x != x ? x : 0.0f);
-    else if constexpr (ACT == QAGG_ACT_SIGMOID)
-    {
-        const float e = expf(-fabsf(x)), d = 1.0f + e;
-        return __fdiv_rn(e, d * d);
-    }
-    else if constexpr (ACT == QAGG_ACT_TANH)
-    {
-        const float e = expf(-2.0f * fabsf(x)), d = 1.0f + e;
-        return __fdiv_rn(4.0f * e, d * d);
-    }
     else if constexpr (ACT == QAGG_ACT_GELU)
-        return __fmaf_rn(x * 0.39894228040143268f, expf(-0.5f * x * x), 0.5f * (1.0f + erff(x * 0.70710678118654752f)));
+    {
+        float e;
+        const float tail = normal_tail(x, e);
+        return __fmaf_rn(x * 0.39894228040143268f, e, x < 0.0f ? tail : 1.0f - tail);
+    }
     else
     {
-        const float e = expf(-fabsf(x)), d = 1.0f + e;
-        const float s = __fdiv_rn(x >= 0.0f ? 1.0f : e, d); // the sigmoid of x
-        return __fmaf_rn(x, __fdiv_rn(e, d * d), s);
+        const float e = exp_minus(ACT == QAGG_ACT_TANH ? 2.0f : 1.0f, x);
+        const float r = rcp_approx(1.0f + e);
+        const float d = e * r * r; // s (1 - s), s the sigmoid of |x| (tanh: of 2 |x|)
+        if constexpr (ACT == QAGG_ACT_SIGMOID)
+            return d;
+        else if constexpr (ACT == QAGG_ACT_TANH)
+            return 4.0f * d;
+        else
+            return __fmaf_rn(x, d, x < 0.0f ? e * r : r);
     }
+}
+
+// Bit pattern, as a float's, of the largest magnitude of a thread's 16 bytes; 16-bit types two at a time.
+template <class T>
+__device__ __forceinline__ unsigned largest16(const uint4& r)
+{
+    if constexpr (sizeof(T) == 4)
+        return max(max(r.x & 0x7fffffffu, r.y & 0x7fffffffu), max(r.z & 0x7fffffffu, r.w & 0x7fffffffu));
+    else
+        return __vmaxu2(__vmaxu2(r.x & 0x7fff7fffu, r.y & 0x7fff7fffu), __vmaxu2(r.z & 0x7fff7fffu, r.w & 0x7fff7fffu));
+}
+template <class T, int THREADS>
+__device__ __forceinline__ unsigned largest_of_block(unsigned top)
+{
+#pragma unroll
+    for (int d = 1; d < THREADS; d *= 2)
+    {
+        const unsigned o = __shfl_xor_sync(0xffffffffu, top, d);
+        top = sizeof(T) == 4 ? max(top, o) : __vmaxu2(top, o);
+    }
+    if constexpr (sizeof(T) == 4)
+        return top;
+    const unsigned t = max(top & 0xffffu, top >> 16);
+    if constexpr (std::is_same_v<T, __nv_bfloat16>)
+        return t << 16;
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short) t)));
 }
 
 // ---- quantize along the rows; with ACT >= 0 also y = f(x) --------------------------------------------------------------------
 
 template <class T, int FMT, int ACT>
-__global__ void __launch_bounds__(MXT) k_mx_quantize(const T* x, long long ldx, unsigned char* codes, unsigned char* scales, T* y, long long ldy,
+__global__ void __launch_bounds__(MXT, 4) k_mx_quantize(const T* x, long long ldx, unsigned char* codes, unsigned char* scales, T* y, long long ldy,
                                                      long long M, long long N, int vecX, int vecY)
 {
+    using S = Shape<T, (ACT >= 0)>;
     __shared__ __align__(16) unsigned char tile[512];
     const long long row0 = (long long) blockIdx.x * MX_TILE;
     const long long col0 = (long long) blockIdx.y * MX_TILE;
-    const int tid = threadIdx.x, seg = tid & 15;
+    const int tid = threadIdx.x, seg = tid % S::LANES, c0 = tid / S::LANES;
     if (tid < 32)
         reinterpret_cast<uint4*>(tile)[tid] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    const long long row = row0 + seg * 8;
-    const int n = row >= M ? 0 : (int) (M - row < 8 ? M - row : 8);
-    const bool block = (row0 + (seg & ~3) * 8) < M; // this thread's block exists
+    const long long row = row0 + seg * S::V;
+    const int n = row >= M ? 0 : (int) (M - row < S::V ? M - row : S::V);
+    const int b = seg * S::V / MX_BLOCK;              // block within the tile
+    const bool block = row0 + b * MX_BLOCK < M;       // it exists
     const long long pitch = mx_pitch(M, FMT);
-    constexpr int HALF = sizeof(T) == 4 ? MX_PASSES / 2 : MX_PASSES; // loads in flight per thread: 64 bytes and up
-#pragma unroll
-    for (int h = 0; h < MX_PASSES; h += HALF)
+    const T* px = x + (col0 + c0) * ldx + row;
+    T* py = y + (col0 + c0) * ldy + row;
+    unsigned char* pc = codes + (col0 + c0) * pitch + (FMT == QAGG_MXFP4 ? row / 2 : row);
+    const int cols = (int) (N - col0 - c0 < MX_TILE ? N - col0 - c0 : MX_TILE); // columns from this thread's first on
+#pragma unroll 1
+    for (int h = 0; h < MX_TILE; h += S::FLIGHT * S::COLS)
     {
-        Raw8<T> raw[HALF];
+        uint4 raw[S::FLIGHT];
 #pragma unroll
-        for (int p = 0; p < HALF; ++p)
+        for (int p = 0; p < S::FLIGHT; ++p)
+            raw[p] = load16(px + p * S::COLS * ldx, h + p * S::COLS < cols ? n : 0, vecX);
+#pragma unroll
+        for (int p = 0; p < S::FLIGHT; ++p)
         {
-            const long long col = col0 + (h + p) * MX_PASS + (tid >> 4);
-            raw[p] = load8(x + col * ldx + row, col < N ? n : 0, vecX);
-        }
-#pragma unroll
-        for (int p = 0; p < HALF; ++p)
-        {
-            const int c = (h + p) * MX_PASS + (tid >> 4);
-            const long long col = col0 + c;
-            float v[8];
-            unpack8(raw[p], v);
-            unsigned top = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const unsigned byte = scale_byte<FMT>(top);
-            if (col < N && block)
+            const int c = h + p * S::COLS; // from this thread's first column
+            float v[S::V];
+            unpack16<T>(raw[p], v);
+            const unsigned byte = scale_byte<FMT>(largest_of_block<T, MX_BLOCK / S::V>(largest16<T>(raw[p])));
+            if (c < cols && block)
             {
-                unsigned w[FMT == QAGG_MXFP4 ? 1 : 2];
-                encode<FMT, 8>(v, byte, w);
-                unsigned char* at = codes + col * pitch + (FMT == QAGG_MXFP4 ? row / 2 : row);
-                if constexpr (FMT == QAGG_MXFP4)
+                const float inv = mx_scale_inv(byte);
+                unsigned w[2];
+#pragma unroll
+                for (int q = 0; q < S::V / 4; ++q)
+                    w[q] = byte == 255u ? 0u : encode4<FMT>(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3], inv);
+                unsigned char* at = pc + p * S::COLS * pitch;
+                if constexpr (FMT == QAGG_MXFP4 && S::V == 4)
+                    *reinterpret_cast<unsigned short*>(at) = (unsigned short) w[0];
+                else if constexpr (FMT == QAGG_MXFP4)
+                    *reinterpret_cast<unsigned*>(at) = w[0] | w[1] << 16;
+                else if constexpr (S::V == 4)
                     *reinterpret_cast<unsigned*>(at) = w[0];
                 else
                     *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
-                if ((seg & 3) == 0)
-                    tile[(c & 31) * 16 + (c >> 5) * 4 + (seg >> 2)] = (unsigned char) byte;
+                if (seg % (MX_BLOCK / S::V) == 0)
+                    tile[((c0 + c) & 31) * 16 + ((c0 + c) >> 5) * 4 + b] = (unsigned char) byte;
                 if constexpr (ACT >= 0)
                 {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        v[i] = act_value<ACT>(v[i]);
-                    store8(y + col * ldy + row, v, n, vecY);
+                    for (int i = 0; i < S::V; ++i)
+                        v[i] = act_value<ACT, T>(v[i]);
+                    store16(py + p * S::COLS * ldy, v, n, vecY);
                 }
             }
         }
+        px += S::FLIGHT * S::COLS * ldx;
+        py += S::FLIGHT * S::COLS * ldy;
+        pc += S::FLIGHT * S::COLS * pitch;
     }
     __syncthreads();
     if (tid < 32)
@@ -255,6 +335,7 @@ __global__ void __launch_bounds__(MXT) k_mx_quantize_t(const T* __restrict__ x, 
 {
     extern __shared__ __align__(16) unsigned char smem[];
     T* s = reinterpret_cast<T*>(smem);
+    auto at = [](int c) { return c * MX_TILE + c / MX_BLOCK * 8; }; // columns of one block 8 values further: see below
     __shared__ __align__(16) unsigned char tile[512];
     const long long col0 = (long long) blockIdx.x * MX_TILE; // columns of x: the packed matrix's rows
     const long long row0 = (long long) blockIdx.y * MX_TILE; // rows of x: the packed matrix's columns
@@ -262,15 +343,15 @@ __global__ void __launch_bounds__(MXT) k_mx_quantize_t(const T* __restrict__ x, 
     if (tid < 32)
         reinterpret_cast<uint4*>(tile)[tid] = make_uint4(0, 0, 0, 0);
     {
-        const int seg = tid & 15;
-        const long long row = row0 + seg * 8;
-        const int n = row >= M ? 0 : (int) (M - row < 8 ? M - row : 8);
+        using S = Shape<T>;
+        const int seg = tid % S::LANES;
+        const long long row = row0 + seg * S::V;
+        const int n = row >= M ? 0 : (int) (M - row < S::V ? M - row : S::V);
 #pragma unroll
-        for (int p = 0; p < MX_PASSES; ++p)
+        for (int p = 0; p < S::PASSES; ++p)
         {
-            const int c = p * MX_PASS + (tid >> 4);
-            const Raw8<T> r = load8(x + (col0 + c) * ldx + row, col0 + c < N ? n : 0, vecX);
-            *reinterpret_cast<Raw8<T>*>(s + c * MX_TILE + seg * 8) = r;
+            const int c = p * S::COLS + tid / S::LANES;
+            *reinterpret_cast<uint4*>(s + at(c) + seg * S::V) = load16(x + (col0 + c) * ldx + row, col0 + c < N ? n : 0, vecX);
         }
     }
     __syncthreads();
@@ -278,7 +359,7 @@ __global__ void __launch_bounds__(MXT) k_mx_quantize_t(const T* __restrict__ x, 
 #pragma unroll 1
     for (int u = tid; u < MX_TILE * 4; u += MXT)
     {
-        const int r = u & (MX_TILE - 1), b = u / MX_TILE;
+        const int r = u >> 2, b = u & 3; // four lanes: 64 (int8: 128) neighbouring bytes; eight rows, four blocks: different banks
         if (row0 + r >= M || col0 + b * MX_BLOCK >= N)
             continue;
         float v[32];
@@ -286,16 +367,23 @@ __global__ void __launch_bounds__(MXT) k_mx_quantize_t(const T* __restrict__ x, 
 #pragma unroll
         for (int i = 0; i < 32; ++i)
         {
-            v[i] = to_float(s[(b * MX_BLOCK + i) * MX_TILE + r]);
+            v[i] = to_float(s[at(b * MX_BLOCK + i) + r]);
             top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
         }
         const unsigned byte = scale_byte<FMT>(top);
-        unsigned w[FMT == QAGG_MXFP4 ? 4 : 8];
-        encode<FMT, 32>(v, byte, w);
-        uint4* at = reinterpret_cast<uint4*>(codes + (row0 + r) * pitch + (col0 + b * MX_BLOCK) / (FMT == QAGG_MXFP4 ? 2 : 1));
-        at[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        if constexpr (FMT == QAGG_MXINT8)
-            at[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        const float inv = mx_scale_inv(byte);
+        unsigned w[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            w[q] = byte == 255u ? 0u : encode4<FMT>(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3], inv);
+        uint4* to = reinterpret_cast<uint4*>(codes + (row0 + r) * pitch + (col0 + b * MX_BLOCK) / (FMT == QAGG_MXFP4 ? 2 : 1));
+        if constexpr (FMT == QAGG_MXFP4)
+            to[0] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+        else
+        {
+            to[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            to[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        }
         tile[(r & 31) * 16 + (r >> 5) * 4 + b] = (unsigned char) byte;
     }
     __syncthreads();
@@ -306,62 +394,82 @@ __global__ void __launch_bounds__(MXT) k_mx_quantize_t(const T* __restrict__ x, 
 // ---- unquantize; with ACT >= 0 the backward pass of a pointwise layer: out = in * f'(value) ----------------------------------
 
 template <class T, int FMT, int ACT>
-__global__ void __launch_bounds__(MXT) k_mx_unquantize(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales, const T* in,
+__global__ void __launch_bounds__(MXT, 4) k_mx_unquantize(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales, const T* in,
                                                        long long ldin, T* out, long long ldout, long long M, long long N, int vecIn, int vecOut)
 {
+    using S = Shape<T, (ACT >= 0)>;
     __shared__ __align__(16) unsigned char tile[512];
     const long long row0 = (long long) blockIdx.x * MX_TILE;
     const long long col0 = (long long) blockIdx.y * MX_TILE;
-    const int tid = threadIdx.x, seg = tid & 15;
-    const long long row = row0 + seg * 8;
-    const int n = row >= M ? 0 : (int) (M - row < 8 ? M - row : 8);
+    const int tid = threadIdx.x, seg = tid % S::LANES, c0 = tid / S::LANES;
+    const long long row = row0 + seg * S::V;
+    const int n = row >= M ? 0 : (int) (M - row < S::V ? M - row : S::V);
+    const int b = seg * S::V / MX_BLOCK;
     const long long pitch = mx_pitch(M, FMT);
-    constexpr int W = FMT == QAGG_MXFP4 ? 1 : 2;
-    constexpr int HALF = sizeof(T) == 4 && ACT >= 0 ? MX_PASSES / 2 : MX_PASSES;
+    const unsigned char* pc = codes + (col0 + c0) * pitch + (FMT == QAGG_MXFP4 ? row / 2 : row);
+    const T* pi = in + (col0 + c0) * ldin + row;
+    T* po = out + (col0 + c0) * ldout + row;
+    const int cols = n == 0 ? 0 : (int) (N - col0 - c0 < MX_TILE ? N - col0 - c0 : MX_TILE);
     if (tid < 32)
         reinterpret_cast<uint4*>(tile)[tid] = __ldcs(reinterpret_cast<const uint4*>(scales + ((long long) blockIdx.y * gridDim.x + blockIdx.x) * 512) + tid);
     __syncthreads();
-#pragma unroll
-    for (int h = 0; h < MX_PASSES; h += HALF)
+#pragma unroll 1
+    for (int h = 0; h < MX_TILE; h += S::FLIGHT * S::COLS)
     {
-        unsigned w[HALF][W];
-        Raw8<T> raw[ACT >= 0 ? HALF : 1];
+        unsigned w[S::FLIGHT][2];
+        uint4 raw[ACT >= 0 ? S::FLIGHT : 1];
 #pragma unroll
-        for (int p = 0; p < HALF; ++p)
+        for (int p = 0; p < S::FLIGHT; ++p)
         {
-            const long long col = col0 + (h + p) * MX_PASS + (tid >> 4);
-            const bool have = col < N && n > 0;
-            const unsigned char* at = codes + col * pitch + (FMT == QAGG_MXFP4 ? row / 2 : row);
-            if constexpr (FMT == QAGG_MXFP4)
-                w[p][0] = have ? __ldcs(reinterpret_cast<const unsigned*>(at)) : 0u;
-            else
+            const bool have = h + p * S::COLS < cols;
+            const unsigned char* at = pc + p * S::COLS * pitch;
+            w[p][0] = w[p][1] = 0;
+            if (have)
             {
-                const uint2 q = have ? __ldcs(reinterpret_cast<const uint2*>(at)) : make_uint2(0, 0);
-                w[p][0] = q.x;
-                w[p][1] = q.y;
+                if constexpr (FMT == QAGG_MXFP4 && S::V == 4)
+                    w[p][0] = __ldcs(reinterpret_cast<const unsigned short*>(at));
+                else if constexpr (FMT == QAGG_MXFP4)
+                {
+                    const unsigned q = __ldcs(reinterpret_cast<const unsigned*>(at));
+                    w[p][0] = q & 0xffffu;
+                    w[p][1] = q >> 16;
+                }
+                else if constexpr (S::V == 4)
+                    w[p][0] = __ldcs(reinterpret_cast<const unsigned*>(at));
+                else
+                {
+                    const uint2 q = __ldcs(reinterpret_cast<const uint2*>(at));
+                    w[p][0] = q.x;
+                    w[p][1] = q.y;
+                }
             }
             if constexpr (ACT >= 0)
-                raw[p] = load8(in + col * ldin + row, have ? n : 0, vecIn);
+                raw[p] = load16(pi + p * S::COLS * ldin, have ? n : 0, vecIn);
         }
 #pragma unroll
-        for (int p = 0; p < HALF; ++p)
+        for (int p = 0; p < S::FLIGHT; ++p)
         {
-            const int c = (h + p) * MX_PASS + (tid >> 4);
-            const long long col = col0 + c;
-            if (col >= N || n == 0)
+            const int c = h + p * S::COLS;
+            if (c >= cols)
                 continue;
-            float v[8];
-            decode8<FMT>(w[p], tile[(c & 31) * 16 + (c >> 5) * 4 + (seg >> 2)], v);
+            const float s = block_scale(tile[((c0 + c) & 31) * 16 + ((c0 + c) >> 5) * 4 + b]);
+            float v[S::V];
+#pragma unroll
+            for (int q = 0; q < S::V / 4; ++q)
+                decode4<FMT>(w[p][q], s, v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
             if constexpr (ACT >= 0)
             {
-                float g[8];
-                unpack8(raw[p], g);
+                float g[S::V];
+                unpack16<T>(raw[p], g);
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
+                for (int i = 0; i < S::V; ++i)
                     v[i] = g[i] * act_slope<ACT>(v[i]);
             }
-            store8(out + col * ldout + row, v, n, vecOut);
+            store16(po + p * S::COLS * ldout, v, n, vecOut);
         }
+        pc += S::FLIGHT * S::COLS * pitch;
+        pi += S::FLIGHT * S::COLS * ldin;
+        po += S::FLIGHT * S::COLS * ldout;
     }
 }
 
@@ -403,7 +511,7 @@ static cudaError_t launch_quantize(cudaStream_t st, const T* x, long long ld, vo
         k_mx_quantize<T, FMT, -1><<<tile_grid(M, N), MXT, 0, st>>>(x, ld, (unsigned char*) codes, (unsigned char*) scales, nullptr, 0, M, N, vec, 0);
     else
     {
-        constexpr int bytes = MX_TILE * MX_TILE * (int) sizeof(T);
+        constexpr int bytes = (MX_TILE * MX_TILE + 32) * (int) sizeof(T);
         if (bytes > 48 * 1024 - 512)
         {
             const cudaError_t e = cudaFuncSetAttribute(k_mx_quantize_t<T, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
