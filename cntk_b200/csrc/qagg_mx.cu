@@ -22,7 +22,7 @@ struct Shape // of the threads over a tile; ACT: with a function's arithmetic, w
     static constexpr int LANES = MX_TILE / V;            // threads per column
     static constexpr int COLS = MXT / LANES;             // columns per pass
     static constexpr int PASSES = MX_TILE / COLS;
-    static constexpr int FLIGHT = ACT ? 4 : 8; // passes whose loads are in flight together
+    static constexpr int FLIGHT = ACT ? 2 : 8; // passes whose loads are in flight together
 };
 
 __device__ __forceinline__ float to_float(float v) { return v; }
@@ -93,49 +93,105 @@ __device__ __forceinline__ unsigned scale_byte(unsigned top)
     return FMT == QAGG_MXFP4 ? (e > 2u ? e - 2u : 0u) : e;
 }
 
-// x / 2^X is exact (a value whose quotient is subnormal is far below the first rounding border).  int8: q by adding 1.5 * 2^23,
-// which rounds to an integer, ties to even, in the low bits.  fp4: the hardware's conversion, nearest even, held at 6.
+// A block's scale as its elements need it.  int8: q is the low byte of x * 2^(6 - X) + 1.5 * 2^23, whose one rounding is to the integer,
+// nearest even; where 2^(6 - X) is no float, or the largest element would round up to 128, the quotient is taken first and held.
+// fp4: the hardware's conversion of x / 2^X (exact), nearest even, held at 6.
 template <int FMT>
-__device__ __forceinline__ unsigned encode4(float a, float b, float c, float d, float inv) // four int8 or (in 16 bits) four fp4 codes
+struct BlockEncoder
 {
-    if constexpr (FMT == QAGG_MXFP4)
-        return (unsigned) __nv_cvt_float2_to_fp4x2(make_float2(a * inv, b * inv), __NV_E2M1, cudaRoundNearest) |
-               (unsigned) __nv_cvt_float2_to_fp4x2(make_float2(c * inv, d * inv), __NV_E2M1, cudaRoundNearest) << 8;
-    else
+    float inv; // 1 / 2^X, int8: 2^(6 - X)
+    bool rare, bad;
+    unsigned byte;
+    __device__ __forceinline__ explicit BlockEncoder(unsigned top)
     {
-        const float v[4] = {a, b, c, d};
+        byte = scale_byte<FMT>(top);
+        bad = byte == 255u;
+        if constexpr (FMT == QAGG_MXFP4)
+        {
+            inv = mx_scale_inv(byte);
+            rare = false;
+        }
+        else
+        {
+            rare = byte < 6u || (top & 0x7f0000u) == 0x7f0000u; // (top: also of NaN and infinity, whose byte is 255)
+            inv = rare || bad ? mx_scale_inv(byte) : __uint_as_float((260u - byte) << 23);
+        }
+    }
+    // four int8 or (in 16 bits) four fp4 codes
+    __device__ __forceinline__ unsigned encode4(float a, float b, float c, float d) const
+    {
+        if (bad)
+            return 0u;
+        if constexpr (FMT == QAGG_MXFP4)
+            return (unsigned) __nv_cvt_float2_to_fp4x2(make_float2(a * inv, b * inv), __NV_E2M1, cudaRoundNearest) |
+                   (unsigned) __nv_cvt_float2_to_fp4x2(make_float2(c * inv, d * inv), __NV_E2M1, cudaRoundNearest) << 8;
+        float v[4] = {a, b, c, d};
+        float scale = inv;
+        if (rare)
+        {
+            asm volatile(""); // a branch
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                v[i] = fminf(fmaxf(v[i] * inv, -127.0f / 64.0f), 127.0f / 64.0f);
+            scale = 64.0f;
+        }
         unsigned q[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            q[i] = __float_as_uint(__fmaf_rn(fminf(fmaxf(v[i] * inv, -127.0f / 64.0f), 127.0f / 64.0f), 64.0f, 12582912.0f));
+            q[i] = __float_as_uint(__fmaf_rn(v[i], scale, 12582912.0f));
         return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
     }
-}
-// four codes -> values; s: the block's scale, NaN for a bad block
+};
+// Codes -> values.  int8: a code with its sign bit turned, set under the exponent of 2^23, is the float 2^23 + 128 + q; times 2^(X - 6) less
+// (2^23 + 128) 2^(X - 6) in one fused step it is the value, exactly.  Where that difference overflows (X > 103, or NaN: s is then NaN in
+// either form) 2^23 + 128 is taken off first.
 template <int FMT>
-__device__ __forceinline__ void decode4(unsigned w, float s, float& a, float& b, float& c, float& d)
+struct BlockDecoder
 {
-    if constexpr (FMT == QAGG_MXFP4)
+    float s, off;
+    bool rare;
+    __device__ __forceinline__ explicit BlockDecoder(unsigned byte)
     {
-        const float2 lo = __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t) (w & 0xffu), __NV_E2M1)));
-        const float2 hi = __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t) (w >> 8 & 0xffu), __NV_E2M1)));
-        a = lo.x * s, b = lo.y * s, c = hi.x * s, d = hi.y * s;
+        if constexpr (FMT == QAGG_MXFP4)
+            s = mx_scale(byte);
+        else
+        {
+            s = byte > 6u ? __uint_as_float((byte - 6u) << 23) : __uint_as_float(0x10000u << byte); // subnormal below byte 7
+            off = s * -8388736.0f;
+        }
+        if (byte == 255u)
+            s = __uint_as_float(0x7fffffffu);
+        rare = byte > 230u;
     }
-    else
+    __device__ __forceinline__ void decode4(unsigned w, float (&v)[4]) const
     {
-        // q by way of 2^23 + 128 + q (an integer in the low bits); element first, then the scale: q / 64 * 2^X, each product exact, down
-        // to the smallest scale
-        const unsigned u = w ^ 0x80808080u;
-        a = __fmaf_rn(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)), 0.015625f, -131074.0f) * s;
-        b = __fmaf_rn(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441)), 0.015625f, -131074.0f) * s;
-        c = __fmaf_rn(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)), 0.015625f, -131074.0f) * s;
-        d = __fmaf_rn(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443)), 0.015625f, -131074.0f) * s;
+        if constexpr (FMT == QAGG_MXFP4)
+        {
+            const float2 lo = __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t) (w & 0xffu), __NV_E2M1)));
+            const float2 hi = __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t) (w >> 8 & 0xffu), __NV_E2M1)));
+            v[0] = lo.x * s, v[1] = lo.y * s, v[2] = hi.x * s, v[3] = hi.y * s;
+        }
+        else
+        {
+            const unsigned u = w ^ 0x80808080u;
+            const float f[4] = {__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441)),
+                                __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443))};
+            if (rare)
+            {
+                asm volatile(""); // a branch: not four more instructions for everybody
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    v[i] = (f[i] - 8388736.0f) * s;
+            }
+            else
+            {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    v[i] = __fmaf_rn(f[i], s, off);
+            }
+        }
     }
-}
-__device__ __forceinline__ float block_scale(unsigned byte)
-{
-    return byte == 255u ? __uint_as_float(0x7fffffffu) : mx_scale(byte);
-}
+};
 
 // ---- pointwise functions -----------------------------------------------------------------------------------------------------
 // In fp32 whatever the type, within about 1e-7 * (1 + |x|): with the hardware's exponential and reciprocal, whose errors of a few
@@ -192,7 +248,7 @@ __device__ __forceinline__ float act_value(float x)
     {
         float e;
         const float tail = normal_tail(x, e);
-        return __fmaf_rn(-fabsf(x), tail, x > 0.0f ? x : x * 0.0f); // x - x tail or x tail; NaN stays
+        return __fmaf_rn(-fabsf(x), tail, fmaxf(x, 0.0f)); // x - x tail or x tail (NaN: tail is)
     }
     else
     {
@@ -256,7 +312,7 @@ __device__ __forceinline__ unsigned largest_of_block(unsigned top)
 // ---- quantize along the rows; with ACT >= 0 also y = f(x) --------------------------------------------------------------------
 
 template <class T, int FMT, int ACT>
-__global__ void __launch_bounds__(MXT, 4) k_mx_quantize(const T* x, long long ldx, unsigned char* codes, unsigned char* scales, T* y, long long ldy,
+__global__ void __launch_bounds__(MXT, (ACT >= 0 ? 5 : 4)) k_mx_quantize(const T* x, long long ldx, unsigned char* codes, unsigned char* scales, T* y, long long ldy,
                                                      long long M, long long N, int vecX, int vecY)
 {
     using S = Shape<T, (ACT >= 0)>;
@@ -289,14 +345,13 @@ __global__ void __launch_bounds__(MXT, 4) k_mx_quantize(const T* x, long long ld
             const int c = h + p * S::COLS; // from this thread's first column
             float v[S::V];
             unpack16<T>(raw[p], v);
-            const unsigned byte = scale_byte<FMT>(largest_of_block<T, MX_BLOCK / S::V>(largest16<T>(raw[p])));
+            const BlockEncoder<FMT> enc(largest_of_block<T, MX_BLOCK / S::V>(largest16<T>(raw[p])));
             if (c < cols && block)
             {
-                const float inv = mx_scale_inv(byte);
                 unsigned w[2];
 #pragma unroll
                 for (int q = 0; q < S::V / 4; ++q)
-                    w[q] = byte == 255u ? 0u : encode4<FMT>(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3], inv);
+                    w[q] = enc.encode4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
                 unsigned char* at = pc + p * S::COLS * pitch;
                 if constexpr (FMT == QAGG_MXFP4 && S::V == 4)
                     *reinterpret_cast<unsigned short*>(at) = (unsigned short) w[0];
@@ -307,7 +362,7 @@ __global__ void __launch_bounds__(MXT, 4) k_mx_quantize(const T* x, long long ld
                 else
                     *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
                 if (seg % (MX_BLOCK / S::V) == 0)
-                    tile[((c0 + c) & 31) * 16 + ((c0 + c) >> 5) * 4 + b] = (unsigned char) byte;
+                    tile[((c0 + c) & 31) * 16 + ((c0 + c) >> 5) * 4 + b] = (unsigned char) enc.byte;
                 if constexpr (ACT >= 0)
                 {
 #pragma unroll
@@ -337,8 +392,10 @@ __global__ void __launch_bounds__(MXT) k_mx_quantize_t(const T* __restrict__ x, 
     T* s = reinterpret_cast<T*>(smem);
     auto at = [](int c) { return c * MX_TILE + c / MX_BLOCK * 8; }; // columns of one block 8 values further: see below
     __shared__ __align__(16) unsigned char tile[512];
-    const long long col0 = (long long) blockIdx.x * MX_TILE; // columns of x: the packed matrix's rows
-    const long long row0 = (long long) blockIdx.y * MX_TILE; // rows of x: the packed matrix's columns
+    // neighbouring CTAs take neighbouring rows of x, which lie together in memory
+    const long long tilesR = (M + MX_TILE - 1) / MX_TILE, tileR = blockIdx.x % tilesR, tileC = blockIdx.x / tilesR;
+    const long long col0 = tileC * MX_TILE; // columns of x: the packed matrix's rows
+    const long long row0 = tileR * MX_TILE; // rows of x: the packed matrix's columns
     const int tid = threadIdx.x;
     if (tid < 32)
         reinterpret_cast<uint4*>(tile)[tid] = make_uint4(0, 0, 0, 0);
@@ -370,12 +427,11 @@ __global__ void __launch_bounds__(MXT) k_mx_quantize_t(const T* __restrict__ x, 
             v[i] = to_float(s[at(b * MX_BLOCK + i) + r]);
             top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
         }
-        const unsigned byte = scale_byte<FMT>(top);
-        const float inv = mx_scale_inv(byte);
+        const BlockEncoder<FMT> enc(top);
         unsigned w[8];
 #pragma unroll
         for (int q = 0; q < 8; ++q)
-            w[q] = byte == 255u ? 0u : encode4<FMT>(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3], inv);
+            w[q] = enc.encode4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
         uint4* to = reinterpret_cast<uint4*>(codes + (row0 + r) * pitch + (col0 + b * MX_BLOCK) / (FMT == QAGG_MXFP4 ? 2 : 1));
         if constexpr (FMT == QAGG_MXFP4)
             to[0] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
@@ -384,17 +440,17 @@ __global__ void __launch_bounds__(MXT) k_mx_quantize_t(const T* __restrict__ x, 
             to[0] = make_uint4(w[0], w[1], w[2], w[3]);
             to[1] = make_uint4(w[4], w[5], w[6], w[7]);
         }
-        tile[(r & 31) * 16 + (r >> 5) * 4 + b] = (unsigned char) byte;
+        tile[(r & 31) * 16 + (r >> 5) * 4 + b] = (unsigned char) enc.byte;
     }
     __syncthreads();
     if (tid < 32)
-        reinterpret_cast<uint4*>(scales + ((long long) blockIdx.y * gridDim.x + blockIdx.x) * 512)[tid] = reinterpret_cast<const uint4*>(tile)[tid];
+        reinterpret_cast<uint4*>(scales + (tileR * mx_scale_tiles(N) + tileC) * 512)[tid] = reinterpret_cast<const uint4*>(tile)[tid];
 }
 
 // ---- unquantize; with ACT >= 0 the backward pass of a pointwise layer: out = in * f'(value) ----------------------------------
 
 template <class T, int FMT, int ACT>
-__global__ void __launch_bounds__(MXT, 4) k_mx_unquantize(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales, const T* in,
+__global__ void __launch_bounds__(MXT, (ACT >= 0 ? 5 : 4)) k_mx_unquantize(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales, const T* in,
                                                        long long ldin, T* out, long long ldout, long long M, long long N, int vecIn, int vecOut)
 {
     using S = Shape<T, (ACT >= 0)>;
@@ -452,11 +508,11 @@ __global__ void __launch_bounds__(MXT, 4) k_mx_unquantize(const unsigned char* _
             const int c = h + p * S::COLS;
             if (c >= cols)
                 continue;
-            const float s = block_scale(tile[((c0 + c) & 31) * 16 + ((c0 + c) >> 5) * 4 + b]);
+            const BlockDecoder<FMT> dec(tile[((c0 + c) & 31) * 16 + ((c0 + c) >> 5) * 4 + b]);
             float v[S::V];
 #pragma unroll
             for (int q = 0; q < S::V / 4; ++q)
-                decode4<FMT>(w[p][q], s, v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                dec.decode4(w[p][q], reinterpret_cast<float(&)[4]>(v[4 * q]));
             if constexpr (ACT >= 0)
             {
                 float g[S::V];
@@ -518,7 +574,8 @@ static cudaError_t launch_quantize(cudaStream_t st, const T* x, long long ld, vo
             if (e != cudaSuccess)
                 return e;
         }
-        k_mx_quantize_t<T, FMT><<<tile_grid(N, M), MXT, bytes, st>>>(x, ld, (unsigned char*) codes, (unsigned char*) scales, M, N, vec);
+        const dim3 tiles = tile_grid(N, M);
+        k_mx_quantize_t<T, FMT><<<tiles.x * tiles.y, MXT, bytes, st>>>(x, ld, (unsigned char*) codes, (unsigned char*) scales, M, N, vec);
     }
     return cudaGetLastError();
 }
