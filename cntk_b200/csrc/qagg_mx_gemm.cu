@@ -22,6 +22,7 @@
 #include "qagg_tcgen05.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <cstring>
 #include <string>
 
@@ -692,12 +693,24 @@ __device__ __forceinline__ void split8(const Raw8<T>& raw, unsigned (&w)[NP][4])
 template <class T>
 __device__ __forceinline__ bool any_special(const Raw8<T>& raw)
 {
-    const T* e = reinterpret_cast<const T*>(&raw);
-    float zero = 0.0f; // stays 0 unless a value is infinite or NaN
+    if constexpr (sizeof(T) == 2)
+    {
+        const __half2* e = reinterpret_cast<const __half2*>(&raw);
+        __half2 zero = __float2half2_rn(0.0f); // stays 0 unless a value is infinite or NaN
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        zero = __fmaf_rn((float) e[i], 0.0f, zero);
-    return zero != 0.0f;
+        for (int i = 0; i < 4; ++i)
+            zero = __hfma2(e[i], __float2half2_rn(0.0f), zero);
+        return (*reinterpret_cast<const unsigned*>(&zero) & 0x7fff7fffu) != 0u;
+    }
+    else
+    {
+        const float* e = reinterpret_cast<const float*>(&raw);
+        float zero = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            zero = __fmaf_rn(e[i], 0.0f, zero);
+        return zero != 0.0f;
+    }
 }
 
 // WEIGHT: dw, lanes = i, columns = o, contraction over the tokens; the dense operand is MN-major (o runs fastest).
@@ -772,46 +785,46 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
         early = count < S ? count : S;
         __syncwarp();
     }
-    // Loaders of the dense operand: rows of 64 contiguous values (128 bytes a plane), in units of eight values, two a thread and step.
-    constexpr int THREADS = DENSE ? 128 * G::load : 1024, UNITS = 1024 / THREADS; // bn <= 128: at most 1024 units
+    // Loaders of the dense operand: rows of 64 contiguous values (128 bytes a plane), in units of eight values.  A thread has two units a
+    // step, the second 64 columns (rows of 64 tokens) further: 8192 bytes in the stage, a constant in memory.
+    constexpr int THREADS = DENSE ? 128 * G::load : 512;
+    static_assert(THREADS * 2 == GRAD_WIDEST_DENSE * 8, "two units a thread");
     struct Units
     {
-        Raw8<TD> raw[UNITS];
+        Raw8<TD> raw[2];
     };
-    const TD* dy = (const TD*) a.dy;
-    const int t = threadIdx.x - G::firstLoad * 32;
-    const long long stepStride = WEIGHT ? GK * a.ldDy : GK;
-    const TD* from[UNITS]; // the unit's next values
-    int have[UNITS];       // WEIGHT: how many of its eight columns exist; otherwise whether its token does
-    int left = 0;          // contraction values from the next step on
+    const int unit = threadIdx.x - G::firstLoad * 32; // 8 row + piece of the row
+    const long long unitStride = WEIGHT ? 64 : 64 * a.ldDy, stepStride = WEIGHT ? GK * a.ldDy : GK;
+    const TD* from = nullptr;       // the first unit's next values
+    int have0 = 0, have1 = 0;       // WEIGHT: how many of the units' eight columns exist; otherwise eight where their token does
+    int left = 0;                   // contraction values from this thread's next one on
     int nextTile = firstTile, nextStep = 0;
     auto fetch = [&](Units& v) { // the next step that this CTA has
         if (nextTile >= a.tiles || count == 0)
             return;
         if (nextStep == 0)
         {
+            const int c = (unit & 7) * 8, r = unit >> 3;
             const long long n0 = tile_n0(nextTile), k0 = (long long) first * GK;
-            left = (int) (a.C - k0);
-#pragma unroll
-            for (int q = 0; q < UNITS; ++q)
+            const long long line = (WEIGHT ? k0 : n0) + r, col = (WEIGHT ? n0 : k0) + c; // token, output
+            from = (const TD*) a.dy + line * a.ldDy + col;
+            left = (int) (a.C - k0) - (WEIGHT ? r : c);
+            if constexpr (WEIGHT)
             {
-                const int u = t + q * THREADS;
-                const int c = u & 7, r = WEIGHT ? (u >> 3) & 63 : u >> 3, atom = WEIGHT ? u >> 9 : 0;
-                const long long col = (WEIGHT ? n0 + atom * 64 : k0) + c * 8, line = (WEIGHT ? k0 : n0) + r; // output, token
                 const long long cols = a.N - col;
-                from[q] = dy + line * a.ldDy + col;
-                have[q] = u >= bn * 8 ? 0 : WEIGHT ? (cols < 0 ? 0 : cols < 8 ? (int) cols : 8) : line < a.N;
+                have0 = (int) (cols < 0 ? 0 : cols < 8 ? cols : 8);
+                have1 = bn <= 64 || cols <= 64 ? 0 : (int) (cols < 72 ? cols - 64 : 8);
+            }
+            else
+            {
+                have0 = line < a.N ? 8 : 0;
+                have1 = bn > 64 && line + 64 < a.N ? 8 : 0;
             }
         }
-#pragma unroll
-        for (int q = 0; q < UNITS; ++q)
-        {
-            const int u = t + q * THREADS;
-            const int rest = left - (WEIGHT ? (u >> 3) & 63 : (u & 7) * 8);
-            const int n = WEIGHT ? (rest > 0 ? have[q] : 0) : (have[q] ? min(max(rest, 0), 8) : 0);
-            v.raw[q] = load8(from[q], n, a.vec);
-            from[q] += stepStride;
-        }
+        const int most = WEIGHT ? (left > 0 ? 8 : 0) : left < 0 ? 0 : left < 8 ? left : 8;
+        v.raw[0] = load8(from, min(have0, most), a.vec);
+        v.raw[1] = load8(from + unitStride, min(have1, most), a.vec);
+        from += stepStride;
         left -= GK;
         if (++nextStep == count)
         {
@@ -1060,19 +1073,17 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
     {
         // Two steps' values are on their way (behind the fence, which would wait for them) while an earlier one is split and stored.
         registers_down<G::regsLoad>();
+        unsigned char* mine = stage0 + (unit >> 3) * 128 + (((unit & 7) ^ (unit >> 3 & 7)) << 4);
         Ring ring;
         long long done = 0;
         auto put_step = [&](const Units& v) {
             if (done >= S)
                 tc_wait(&bars.empty[ring.s], ring.par ^ 1, &bars.broken, &g_mxStatus);
             ++done;
-            unsigned char* at = stage0 + ring.s * stageBytes;
+            unsigned char* at = mine + ring.s * stageBytes;
 #pragma unroll
-            for (int q = 0; q < UNITS; ++q)
+            for (int q = 0; q < 2; ++q)
             {
-                const int u = t + q * THREADS;
-                const int c = u & 7, r = WEIGHT ? (u >> 3) & 63 : u >> 3, atom = WEIGHT ? u >> 9 : 0;
-                unsigned char* dst = at + atom * 8192 + r * 128 + ((c ^ (r & 7)) << 4);
                 unsigned w[NP][4];
                 if (NP == 1)
                     *reinterpret_cast<uint4*>(w[0]) = v.raw[q].a;
@@ -1080,10 +1091,10 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
                     split8<TD, NP, true>(v.raw[q], w);
                 else
                     split8<TD, NP, false>(v.raw[q], w);
+                if (q == 0 || bn > 64)
 #pragma unroll
-                for (int p = 0; p < NP; ++p)
-                    if (u < bn * 8)
-                        *reinterpret_cast<uint4*>(dst + p * bn * 128) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+                    for (int p = 0; p < NP; ++p)
+                        *reinterpret_cast<uint4*>(at + q * 8192 + p * bn * 128) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
             }
             fence_async_shared();
             __syncwarp();
@@ -1118,13 +1129,14 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
 // ---- launches -----------------------------------------------------------------------------------------------------------------
 
 // Tile width and split of the contraction, by a count of cycles: a CTA runs waves * steps / splits steps, each as long as its products
-// (2 * bn * planes: 8192 bf16 or 32768 fp4 multiply-adds a cycle) or its copies (64 bytes a cycle from L2) take, whichever is more;
-// then the last tile's result goes out.
+// (2 * bn * planes: 8192 bf16 or 32768 fp4 multiply-adds a cycle), its copies (46 bytes a cycle from L2) or its preparation
+// (`least`: expanding a step takes the warps 450 cycles, splitting a dense one 1300) take, whichever is most; then the last tile's
+// result goes out.
 struct Shape
 {
     int bn, splits;
 };
-static Shape choose_shape(long long tilesM, long long N, int steps, int sms, const int* widths, int nWidths, int planes, int fixedBytes, int columnBytes)
+static Shape choose_shape(long long tilesM, long long N, int steps, int sms, const int* widths, int nWidths, int planes, int fixedBytes, int columnBytes, double least)
 {
     Shape best = {widths[0], 1};
     double bestCost = 1e300;
@@ -1134,7 +1146,7 @@ static Shape choose_shape(long long tilesM, long long N, int steps, int sms, con
         if (i > 0 && bn < 128 && N > bn)
             break; // several narrow tiles would read the other operand once each
         const long long tiles = tilesM * ((N + bn - 1) / bn);
-        const double step = 50.0 + std::max(2.0 * bn * planes, (fixedBytes + (double) bn * columnBytes) / 64.0);
+        const double step = 50.0 + std::max(std::max(2.0 * bn * planes, (fixedBytes + (double) bn * columnBytes) / 46.0), least);
         for (int s = 1; s <= 8; s *= 2)
         {
             if (s > 1 && s > steps)
@@ -1162,12 +1174,22 @@ static int smem_for(int stageBytes, int stages, int resultBytes)
     return std::max(GEMM_SMEM_MIN, 1024 + std::max(stageBytes * stages, resultBytes));
 }
 
-template <class K, class... Args>
-static cudaError_t launch_cluster(K kernel, dim3 grid, int threads, int smem, dim3 cluster, cudaStream_t st, Args... args)
+// The kernels' limit of dynamic shared memory is raised once per device.
+template <auto KERNEL, class... Args>
+static cudaError_t launch_cluster(dim3 grid, int threads, int smem, dim3 cluster, cudaStream_t st, Args... args)
 {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<unsigned long long> raised{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess)
         return e;
+    if (!(raised.load(std::memory_order_relaxed) >> dev & 1)) // devices 0..63: launch_cfg_for_current_device has seen to it
+    {
+        e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, GEMM_SMEM_MAX);
+        if (e != cudaSuccess)
+            return e;
+        raised.fetch_or(1ull << dev);
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
@@ -1180,7 +1202,7 @@ static cudaError_t launch_cluster(K kernel, dim3 grid, int threads, int smem, di
     attr[0].val.clusterDim.z = cluster.z;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    e = cudaLaunchKernelEx(&cfg, KERNEL, args...);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
@@ -1199,15 +1221,14 @@ static cudaError_t launch_grad(cudaStream_t st, const CUtensorMap& mc, const CUt
         {
             const int stageBytes = GRAD_PAIR / 2 * 128 + grad_codes_bytes(FMT) + GRAD_SCALE_ROOM;
             a.stages = stages_for(stageBytes, MAX_STAGES);
-            const auto kernel = k_mx_grad<WEIGHT, FMT, 0, true, TD, TO>;
             const int smem = smem_for(stageBytes, a.stages, 0);
-            return launch_cluster(kernel, dim3((unsigned) (2 * std::min(a.tiles, sms / 2))), GradGroups<false, true>::threads, smem, dim3(2, 1, 1), st, mc, md, a);
+            return launch_cluster<k_mx_grad<WEIGHT, FMT, 0, true, TD, TO>>(dim3((unsigned) (2 * std::min(a.tiles, sms / 2))), GradGroups<false, true>::threads, smem, dim3(2, 1, 1), st, mc, md, a);
         }
     const int stageBytes = a.bn * 128 * NP + grad_codes_bytes(FMT) + GRAD_SCALE_ROOM;
     a.stages = stages_for(stageBytes, MAX_STAGES);
     const int smem = smem_for(stageBytes, a.stages, a.splits > 1 ? 128 * (a.bn + 4) * 4 : 0);
     const dim3 grid((unsigned) (a.splits > 1 ? a.tiles : std::min(a.tiles, sms)), 1, (unsigned) a.splits);
-    return launch_cluster(k_mx_grad<WEIGHT, FMT, DENSE, false, TD, TO>, grid, GradGroups<(DENSE > 0), false>::threads, smem, dim3(1, 1, a.splits), st, mc, md, a);
+    return launch_cluster<k_mx_grad<WEIGHT, FMT, DENSE, false, TD, TO>>(grid, GradGroups<(DENSE > 0), false>::threads, smem, dim3(1, 1, a.splits), st, mc, md, a);
 }
 
 template <bool WEIGHT, int FMT, class TO>
@@ -1270,7 +1291,7 @@ static int grad_common(const char* who, bool weight, void* stream, const void* d
     const bool tma = dyType == QAGG_BF16 && a.vec;
     static const int wide[] = {GRAD_WIDEST, GRAD_WIDEST_DENSE, 64};
     const Shape sh = choose_shape((I + 127) / 128, N, (int) ((C + GK - 1) / GK), cfg.numSMs, tma ? wide : wide + 1, tma ? 3 : 2, dyType == QAGG_BF16 ? 1 : dyType == QAGG_F16 ? 2 : 3,
-                                  grad_codes_bytes(format), GK * mx_type_bytes(dyType));
+                                  grad_codes_bytes(format), GK * mx_type_bytes(dyType), tma ? 450.0 : 1300.0);
     a.bn = sh.bn;
     a.splits = sh.splits;
     a.tilesM = (int) ((I + 127) / 128);
@@ -1348,7 +1369,7 @@ int qagg_mx_times(void* stream, const void* w_codes, const void* w_scales, const
     a.T = T;
     a.K = K;
     static const int widths[] = {256, 128, 64, 32, 16};
-    const Shape sh = choose_shape((O + 127) / 128, T, (int) ((K + TK - 1) / TK), cfg.numSMs, widths, 5, 1, 128 * (128 + 8), 128 + 8);
+    const Shape sh = choose_shape((O + 127) / 128, T, (int) ((K + TK - 1) / TK), cfg.numSMs, widths, 5, 1, 128 * (128 + 8), 128 + 8, 0.0);
     a.bn = sh.bn;
     a.splits = sh.splits;
     a.tilesM = (int) ((O + 127) / 128);
@@ -1369,12 +1390,12 @@ int qagg_mx_times(void* stream, const void* w_codes, const void* w_scales, const
     const dim3 cluster(1, 1, a.splits);
     const bool narrow = a.bn <= TIMES_NARROW;
     if (y_type == QAGG_F32)
-        e = narrow ? launch_cluster(k_mx_times<float, TIMES_NARROW>, grid, TT, smem, cluster, st, mw, mx, a) : launch_cluster(k_mx_times<float, 128>, grid, TT, smem, cluster, st, mw, mx, a);
+        e = narrow ? launch_cluster<k_mx_times<float, TIMES_NARROW>>(grid, TT, smem, cluster, st, mw, mx, a) : launch_cluster<k_mx_times<float, 128>>(grid, TT, smem, cluster, st, mw, mx, a);
     else if (y_type == QAGG_F16)
-        e = narrow ? launch_cluster(k_mx_times<__half, TIMES_NARROW>, grid, TT, smem, cluster, st, mw, mx, a) : launch_cluster(k_mx_times<__half, 128>, grid, TT, smem, cluster, st, mw, mx, a);
+        e = narrow ? launch_cluster<k_mx_times<__half, TIMES_NARROW>>(grid, TT, smem, cluster, st, mw, mx, a) : launch_cluster<k_mx_times<__half, 128>>(grid, TT, smem, cluster, st, mw, mx, a);
     else
-        e = narrow ? launch_cluster(k_mx_times<__nv_bfloat16, TIMES_NARROW>, grid, TT, smem, cluster, st, mw, mx, a)
-                   : launch_cluster(k_mx_times<__nv_bfloat16, 128>, grid, TT, smem, cluster, st, mw, mx, a);
+        e = narrow ? launch_cluster<k_mx_times<__nv_bfloat16, TIMES_NARROW>>(grid, TT, smem, cluster, st, mw, mx, a)
+                   : launch_cluster<k_mx_times<__nv_bfloat16, 128>>(grid, TT, smem, cluster, st, mw, mx, a);
     return check_cuda(e, "4-bit product kernel launch");
 }
 
