@@ -25,6 +25,7 @@
 #include <atomic>
 #include <cstring>
 #include <string>
+#include <type_traits>
 
 namespace qagg {
 
@@ -374,25 +375,31 @@ constexpr int TIMES_NARROW = 32;
 constexpr int TK = 256;  // contraction values per stage: 128 bytes of codes
 
 
-__host__ __device__ inline int times_stage_bytes(int bn)
+constexpr int TIMES_PAIR = 256; // width of a tile that two CTAs make
+// codes of 128 rows of W and `rows` of X, scales of W's and of bn of X's
+__host__ __device__ inline int times_stage_bytes(int bn, int rows)
 {
-    return 128 * 128 + bn * 128 + 1024 + (bn > 128 ? 2048 : 1024);
+    return 128 * 128 + rows * 128 + 1024 + (bn > 128 ? 2048 : 1024);
 }
 
 // ACC: most columns of the tile that one result warp holds.  The narrow tiles of few tokens have a kernel of their own, whose results are
 // a quarter of the code: a launch that lasts 3 us feels the instruction fetches (128: 1400 cycles to put the sums down).
-template <class T, int ACC>
+// PAIR: two CTAs make a 256 x 256 tile together, each with half of W's and of X's rows: 35 KB a step for each instead of 51.
+template <class T, int ACC, bool PAIR>
 __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapX, const TimesArgs a)
 {
     extern __shared__ unsigned char dyn[];
     __shared__ GemmBars bars;
     unsigned char* stage0 = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t) 1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int bn = a.bn, S = a.stages, stageBytes = times_stage_bytes(bn);
+    const int bn = a.bn, S = a.stages, share = PAIR ? bn / 2 : bn, stageBytes = times_stage_bytes(bn, share);
+    const unsigned codesBytes = 16384 + share * 128;
     const int steps = (int) ((a.K + TK - 1) / TK);
-    const int rank = a.splits > 1 ? (int) cluster_rank() : 0;
-    int first, count;
-    split_range(steps, rank, a.splits, first, count);
+    const int rank = PAIR || a.splits > 1 ? (int) cluster_rank() : 0;
+    int first = 0, count = steps;
+    if (!PAIR)
+        split_range(steps, rank, a.splits, first, count);
+    const int firstTile = PAIR ? blockIdx.x >> 1 : blockIdx.x, tileStep = PAIR ? gridDim.x >> 1 : gridDim.x;
     const long long chunks = mx_scale_tiles(a.K); // scale tiles along the contraction, 128 values each
     const int resultWarps = bn > 128 ? 8 : 4;
     const int bufs = bn > 128 ? 1 : 2; // accumulators, 128 columns apart
@@ -406,15 +413,18 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
         const unsigned char *scaleW, *scaleX;
     };
     auto source_of = [&](int tile) {
-        const int m = tile % a.tilesM, n0 = tile / a.tilesM * bn;
-        return Source{m * 128, n0, bn > 128 && n0 + 128 < a.T ? 2 : 1, a.scaleW + (long long) m * chunks * 512, a.scaleX + (long long) (n0 / 128) * chunks * 512};
+        const int m = (tile % a.tilesM) * (PAIR ? 2 : 1) + (PAIR ? rank : 0), n0 = tile / a.tilesM * bn;
+        // (a CTA of a pair may have no rows of W: codes outside read as zero, scales are taken from the last rows)
+        const long long rowTile = m * 128LL < a.O ? m : (a.O - 1) / 128;
+        return Source{m * 128, n0 + (PAIR ? rank * share : 0), bn > 128 && n0 + 128 < a.T ? 2 : 1, a.scaleW + rowTile * chunks * 512,
+                      a.scaleX + (long long) (n0 / 128) * chunks * 512};
     };
     auto copy_step = [&](const Source& src, int i, int s) {
-        const unsigned at = smem_addr(stage0) + s * stageBytes, sw = at + 16384 + bn * 128;
+        const unsigned at = smem_addr(stage0) + s * stageBytes, sw = at + codesBytes;
         const int k = first + i;
         const unsigned bytes = chunks - 2 * k < 2 ? 512 : 1024;
         unsigned long long* full = &bars.full[s];
-        mbar_arrive_expect_tx(full, 128 * 128 + bn * 128 + bytes * (1 + src.rowsX));
+        mbar_arrive_expect_tx(full, codesBytes + bytes * (1 + src.rowsX));
         tma_load_2d(at, &mapW, k * 128, src.m0, full);
         tma_load_2d(at + 16384, &mapX, k * 128, src.n0, full);
         bulk_load(sw, src.scaleW + k * 1024LL, bytes, full);
@@ -425,10 +435,10 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
     int early = 0; // steps of the first tile whose copies start before the CTA has met
     if (warp == 0)
     {
-        init_barriers(&bars, S, 1, 1, resultWarps);
+        init_barriers(&bars, S, 1, 1, PAIR ? 2 * resultWarps : resultWarps);
         if (elect_one())
         {
-            const Source src = source_of(blockIdx.x);
+            const Source src = source_of(firstTile);
             for (; early < count && early < S; ++early)
                 copy_step(src, early, early);
         }
@@ -436,9 +446,11 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
         __syncwarp();
     }
     if (warp == 2)
-        tmem_alloc(&bars.tmem, TMEM_COLS);
+        tmem_alloc<PAIR>(&bars.tmem, TMEM_COLS);
     tc_fence_before();
     __syncthreads();
+    if (PAIR)
+        cluster_sync(); // the other CTA's barriers exist
     tc_fence_after();
     const unsigned tm = bars.tmem;
 
@@ -450,10 +462,10 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
             for (int i = 0; i < early; ++i)
                 ring.next(S);
             long long issued = early;
-            for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
+            for (int tile = firstTile; tile < a.tiles; tile += tileStep)
             {
                 const Source src = source_of(tile);
-                for (int i = tile == (int) blockIdx.x ? early : 0; i < count; ++i, ++issued)
+                for (int i = tile == firstTile ? early : 0; i < count; ++i, ++issued)
                 {
                     if (issued >= S)
                         tc_wait(&bars.empty[ring.s], ring.par ^ 1, &bars.broken, &g_mxStatus);
@@ -469,18 +481,18 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
             }
         }
     }
-    else if (warp == 1)
+    else if (warp == 1 && (!PAIR || rank == 0))
     {
         if (elect_one())
         {
             Ring ring;
             Chains chain;
             bool fresh = true; // accumulators that no chain has used
-            const unsigned id0 = idesc_mxf4(bn, 0), id2 = idesc_mxf4(bn, 2);
+            const unsigned id0 = idesc_mxf4(bn, 0, PAIR ? 256 : 128), id2 = idesc_mxf4(bn, 2, PAIR ? 256 : 128);
             const unsigned long long dW = smem_desc(smem_addr(stage0), 16, 1024, SWIZZLE_128B);
             const unsigned long long dX = dW + (16384 >> 4);
-            const unsigned long long dS = smem_desc(smem_addr(stage0) + 16384 + bn * 128, 16, 128, SWIZZLE_NONE);
-            for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
+            const unsigned long long dS = smem_desc(smem_addr(stage0) + codesBytes, 16, 128, SWIZZLE_NONE);
+            for (int tile = firstTile; tile < a.tiles; tile += tileStep)
             {
                 const long long n0 = (long long) (tile / a.tilesM) * bn;
                 const bool twoX = bn > 128 && n0 + 128 < a.T;
@@ -490,6 +502,8 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
                     if (inChain == 0 && !fresh)
                         tc_wait(&bars.taken[chain.buf], chain.par ^ 1, &bars.broken, &g_mxStatus);
                     tc_wait(&bars.full[ring.s], ring.par, &bars.broken, &g_mxStatus);
+                    if (PAIR)
+                        tc_wait(&bars.conv[ring.s], ring.par, &bars.broken, &g_mxStatus); // the other CTA's copies
                     tc_fence_after();
                     const unsigned d = tm + chain.buf * 128;
                     const unsigned long long off = (unsigned long long) (unsigned) (ring.s * stageBytes) >> 4;
@@ -497,34 +511,54 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
                     const unsigned sa = tm + SIDE + ring.s * 24, sb = sa + 8; // eight columns of W's scales, sixteen of X's
                     const long long left = a.K - (long long) (first + i) * TK;
                     const bool more = inChain > 0;
-                    tmem_copy_scales(sa, sc);
-                    tmem_copy_scales(sb, sc + (1024 >> 4));
+                    tmem_copy_scales<PAIR>(sa, sc);
+                    tmem_copy_scales<PAIR>(sb, sc + (1024 >> 4));
                     if (twoX)
-                        tmem_copy_scales(sb + 4, sc + (2048 >> 4));
-                    mma_mxf4_ss(d, w, x, id0, sa, sb, more);
+                        tmem_copy_scales<PAIR>(sb + 4, sc + (2048 >> 4));
+                    mma_mxf4_ss<PAIR>(d, w, x, id0, sa, sb, more);
                     if (left > 64)
-                        mma_mxf4_ss(d, w + 2, x + 2, id2, sa, sb, true);
+                        mma_mxf4_ss<PAIR>(d, w + 2, x + 2, id2, sa, sb, true);
                     if (left > 128)
                     {
-                        tmem_copy_scales(sa + 4, sc + (512 >> 4));
-                        tmem_copy_scales(sb + 8, sc + (1536 >> 4));
+                        tmem_copy_scales<PAIR>(sa + 4, sc + (512 >> 4));
+                        tmem_copy_scales<PAIR>(sb + 8, sc + (1536 >> 4));
                         if (twoX)
-                            tmem_copy_scales(sb + 12, sc + (2560 >> 4));
-                        mma_mxf4_ss(d, w + 4, x + 4, id0, sa + 4, sb + 8, true);
+                            tmem_copy_scales<PAIR>(sb + 12, sc + (2560 >> 4));
+                        mma_mxf4_ss<PAIR>(d, w + 4, x + 4, id0, sa + 4, sb + 8, true);
                         if (left > 192)
-                            mma_mxf4_ss(d, w + 6, x + 6, id2, sa + 4, sb + 8, true);
+                            mma_mxf4_ss<PAIR>(d, w + 6, x + 6, id2, sa + 4, sb + 8, true);
                     }
-                    tc_commit(&bars.empty[ring.s]);
+                    if constexpr (PAIR)
+                        tc_commit_pair(&bars.empty[ring.s]);
+                    else
+                        tc_commit(&bars.empty[ring.s]);
                     ring.next(S);
                     if (++inChain == CHAIN_STEPS || i + 1 == count)
                     {
-                        tc_commit(&bars.ready[chain.buf]);
+                        if constexpr (PAIR)
+                            tc_commit_pair(&bars.ready[chain.buf]);
+                        else
+                            tc_commit(&bars.ready[chain.buf]);
                         chain.next(bufs);
                         fresh = fresh && chain.buf != 0;
                         inChain = 0;
                     }
                 }
             }
+        }
+    }
+    else if (PAIR && warp == 3 && rank == 1)
+    {
+        if (elect_one())
+        {
+            Ring ring; // tells the issuing CTA of the copies that have landed here
+            for (int tile = firstTile; tile < a.tiles; tile += tileStep)
+                for (int i = 0; i < count; ++i)
+                {
+                    tc_wait(&bars.full[ring.s], ring.par, &bars.broken, &g_mxStatus);
+                    mbar_arrive_remote(&bars.conv[ring.s], 0);
+                    ring.next(S);
+                }
         }
     }
     else if (warp >= 4)
@@ -536,12 +570,12 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
             const unsigned mine = tm + ((unsigned) (quad * 32) << 16) + half * 128;
             const int m = quad * 32 + lane;
             Chains chain;
-            for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
+            for (int tile = firstTile; tile < a.tiles; tile += tileStep)
             {
-                const long long m0 = (long long) (tile % a.tilesM) * 128, n0 = (long long) (tile / a.tilesM) * bn;
+                const long long m0 = (long long) (tile % a.tilesM) * (PAIR ? 256 : 128) + (PAIR ? rank * 128 : 0), n0 = (long long) (tile / a.tilesM) * bn;
                 const float bias = a.bias && a.splits == 1 && m0 + m < a.O ? a.bias[m0 + m] : 0.0f;
                 float* buf = reinterpret_cast<float*>(stage0);
-                if (a.tiles <= (int) gridDim.x && count <= CHAIN_STEPS)
+                if (!PAIR && a.tiles <= tileStep && count <= CHAIN_STEPS)
                 {
                     drain_chain(&bars, mine, cols, count == 0, [&](int j, const float(&v)[16]) {
                         if (a.splits > 1)
@@ -556,8 +590,8 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
                 for (int j = 0; j < ACC; ++j)
                     acc[j] = 0.0f;
                 for (int i = 0; i < count; i += CHAIN_STEPS, chain.next(bufs))
-                    take_chain<false>(&bars, chain.buf, chain.par, mine + chain.buf * 128, cols, i == 0, acc);
-                if (a.splits > 1)
+                    take_chain<PAIR>(&bars, chain.buf, chain.par, mine + chain.buf * 128, cols, i == 0, acc);
+                if (!PAIR && a.splits > 1)
                     put_partial<false>(buf, bn, m, half * 128, cols, acc);
                 else
                     write_columns((T*) a.y, a.ld, m0 + m, a.O, n0 + half * 128, a.T, cols, acc, bias, lane ^ 1, a.pairs && m0 + 128 <= a.O);
@@ -565,13 +599,15 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
         }
     }
     __syncwarp();
-    if (a.splits > 1) // one tile per cluster
+    if (!PAIR && a.splits > 1) // one tile per cluster
         reduce_cluster<false, T>(reinterpret_cast<float*>(stage0), a.splits, rank, bn, (T*) a.y, a.ld, (long long) (blockIdx.x % a.tilesM) * 128, a.O,
                                  (long long) (blockIdx.x / a.tilesM) * bn, a.T, a.bias, false, a.wide4);
     tc_fence_before();
+    if (PAIR)
+        cluster_sync(); // neither goes while the other may still arrive at its barriers or use its memory
     __syncthreads();
     if (warp == 2)
-        tmem_free(tm, TMEM_COLS);
+        tmem_free<PAIR>(tm, TMEM_COLS);
 }
 
 // ---- gradients --------------------------------------------------------------------------------------------------------------------
@@ -1376,26 +1412,36 @@ int qagg_mx_times(void* stream, const void* w_codes, const void* w_scales, const
     a.tiles = a.tilesM * (int) ((T + a.bn - 1) / a.bn);
     a.pairs = ((uintptr_t) y & 3) == 0 && (ld_y & 1) == 0;
     a.wide4 = (((uintptr_t) y | (uintptr_t) (ld_y * mx_type_bytes(y_type))) & (4 * mx_type_bytes(y_type) - 1)) == 0;
-    const int stageBytes = times_stage_bytes(a.bn);
+    // two CTAs on a 256 x 256 tile, or one on 128 x bn: cycles as in choose_shape
+    const long long pairs = (O + 255) / 256 * ((T + 255) / 256);
+    const bool pair = a.splits == 1 && 1.05 * 780.0 * ((pairs + cfg.numSMs / 2 - 1) / (cfg.numSMs / 2)) <
+                                           std::max(2.0 * a.bn, (128 + a.bn) * 136.0 / 46.0) * ((a.tiles + cfg.numSMs - 1) / cfg.numSMs);
+    if (pair)
+    {
+        a.bn = TIMES_PAIR;
+        a.tilesM = (int) ((O + 255) / 256);
+        a.tiles = (int) pairs;
+    }
+    const int stageBytes = times_stage_bytes(a.bn, pair ? a.bn / 2 : a.bn);
     a.stages = stages_for(stageBytes, MAX_STAGES);
     const int smem = smem_for(stageBytes, a.stages, a.splits > 1 ? 128 * a.bn * 4 : 0);
     alignas(64) CUtensorMap mw, mx;
     std::memset(&mw, 0, sizeof(mw));
     std::memset(&mx, 0, sizeof(mx));
-    if (K > 0 && (!codes_map(&mw, w_codes, K, O, QAGG_MXFP4, 128, 128) || !codes_map(&mx, x_codes, K, T, QAGG_MXFP4, 128, a.bn)))
+    if (K > 0 && (!codes_map(&mw, w_codes, K, O, QAGG_MXFP4, 128, 128) || !codes_map(&mx, x_codes, K, T, QAGG_MXFP4, 128, pair ? a.bn / 2 : a.bn)))
         return fail(QAGG_ECUDA, "qagg_mx_times: tensor maps of the codes could not be made");
-    const dim3 grid((unsigned) (a.splits > 1 ? a.tiles : std::min(a.tiles, cfg.numSMs)), 1, (unsigned) a.splits);
+    const dim3 grid((unsigned) (pair ? 2 * std::min(a.tiles, cfg.numSMs / 2) : a.splits > 1 ? a.tiles : std::min(a.tiles, cfg.numSMs)), 1, (unsigned) a.splits);
+    const dim3 cluster(pair ? 2 : 1, 1, a.splits);
     const cudaStream_t st = (cudaStream_t) stream;
-    cudaError_t e;
-    const dim3 cluster(1, 1, a.splits);
-    const bool narrow = a.bn <= TIMES_NARROW;
-    if (y_type == QAGG_F32)
-        e = narrow ? launch_cluster<k_mx_times<float, TIMES_NARROW>>(grid, TT, smem, cluster, st, mw, mx, a) : launch_cluster<k_mx_times<float, 128>>(grid, TT, smem, cluster, st, mw, mx, a);
-    else if (y_type == QAGG_F16)
-        e = narrow ? launch_cluster<k_mx_times<__half, TIMES_NARROW>>(grid, TT, smem, cluster, st, mw, mx, a) : launch_cluster<k_mx_times<__half, 128>>(grid, TT, smem, cluster, st, mw, mx, a);
-    else
-        e = narrow ? launch_cluster<k_mx_times<__nv_bfloat16, TIMES_NARROW>>(grid, TT, smem, cluster, st, mw, mx, a)
-                   : launch_cluster<k_mx_times<__nv_bfloat16, 128>>(grid, TT, smem, cluster, st, mw, mx, a);
+    const auto launch = [&](auto* t) {
+        using T_ = std::remove_pointer_t<decltype(t)>;
+        if (pair)
+            return launch_cluster<k_mx_times<T_, 128, true>>(grid, TT, smem, cluster, st, mw, mx, a);
+        if (a.bn <= TIMES_NARROW)
+            return launch_cluster<k_mx_times<T_, TIMES_NARROW, false>>(grid, TT, smem, cluster, st, mw, mx, a);
+        return launch_cluster<k_mx_times<T_, 128, false>>(grid, TT, smem, cluster, st, mw, mx, a);
+    };
+    const cudaError_t e = y_type == QAGG_F32 ? launch((float*) nullptr) : y_type == QAGG_F16 ? launch((__half*) nullptr) : launch((__nv_bfloat16*) nullptr);
     return check_cuda(e, "4-bit product kernel launch");
 }
 

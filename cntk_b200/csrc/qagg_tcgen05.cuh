@@ -158,8 +158,15 @@ __device__ __forceinline__ void tmem_store_wait()
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 // 512 bytes of shared memory (32 rows of 16 bytes) -> 4 columns, repeated in the four groups of 32 lanes: a tile of block scales
+// (PAIR: in each of the two CTAs, from its own shared memory at the same address)
+template <bool PAIR = false>
 __device__ __forceinline__ void tmem_copy_scales(unsigned addr, unsigned long long desc)
 {
+    if constexpr (PAIR)
+    {
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(addr), "l"(desc) : "memory");
+        return;
+    }
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(addr), "l"(desc) : "memory");
 }
 
@@ -179,10 +186,10 @@ __host__ __device__ constexpr unsigned idesc_bf16(int n, bool transB, int m = 12
 {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((transB ? 1u : 0u) << 16) | ((unsigned) (n >> 3) << 17) | ((unsigned) (m >> 4) << 24);
 }
-// e2m1 x e2m1 with one power-of-two scale per 32 values -> fp32, 128 x n; sf: which pair of a scale word's four bytes
-__host__ __device__ constexpr unsigned idesc_mxf4(int n, unsigned sf)
+// e2m1 x e2m1 with one power-of-two scale per 32 values -> fp32, m x n; sf: which pair of a scale word's four bytes
+__host__ __device__ constexpr unsigned idesc_mxf4(int n, unsigned sf, int m = 128)
 {
-    return (sf << 4) | (1u << 7) | (1u << 10) | ((unsigned) (n >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24) | (sf << 29);
+    return (sf << 4) | (1u << 7) | (1u << 10) | ((unsigned) (n >> 3) << 17) | (1u << 23) | ((unsigned) (m >> 4) << 24) | (sf << 29);
 }
 // D (+)= A B, A in tensor memory (16 contraction values in 8 columns), B in shared memory
 __device__ __forceinline__ void mma_bf16_ts(unsigned d, unsigned a, unsigned long long b, unsigned idesc, bool add)
@@ -200,8 +207,19 @@ __device__ __forceinline__ void mma_bf16_ts_pair(unsigned d, unsigned a, unsigne
                  : "memory");
 }
 // D (+)= A B over 64 contraction values, both in shared memory, block scales in tensor memory
+// (PAIR: two CTAs, 256 rows, half of A's and of B's rows in each one's shared memory; the scales of its own 128 rows of A and of all of
+// B's in each one's tensor memory)
+template <bool PAIR = false>
 __device__ __forceinline__ void mma_mxf4_ss(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned scaleA, unsigned scaleB, bool add)
 {
+    if constexpr (PAIR)
+    {
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+                     "r"(scaleA), "r"(scaleB), "r"((unsigned) add)
+                     : "memory");
+        return;
+    }
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
                  "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
                  "r"(scaleA), "r"(scaleB), "r"((unsigned) add)
