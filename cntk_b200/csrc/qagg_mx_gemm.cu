@@ -610,6 +610,165 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
         tmem_free<PAIR>(tm, TMEM_COLS);
 }
 
+// ---- 4-bit product, a few tokens ------------------------------------------------------------------------------------------------
+// Up to four tokens read the weights once and do little with them: no tensor cores, no tensor maps, one short launch.  A warp takes one
+// output row (two where there are enough), a lane every 32nd block of it: 16 bytes, the next ones on their way.  Twice an element is an
+// integer of at most 12, looked up four at a time by PRMT, so a block's products are integer dot products, exact: with mag the
+// magnitudes of w and x signed, sum w x = sum mag x - 2 * (sum over negative w of mag x).  x is decoded once per CTA, into shared
+// memory.  Only the sum over blocks is in fp32.
+// Chosen up to FEW_PRODUCTS multiply-adds: beyond them its instructions last longer than what the tiles need besides the weights.
+// us, this / tiles:  2048 x 2048, 1 token 2.6 / 4.9, 4 tokens 4.2 / 5.3;  9304 x 4096, 1 token 7.3 / 7.5, 4 tokens 14.8 / 7.5.
+constexpr int FEW = 4, FEW_VALUES = 32768; // tokens; values of x, a byte each in shared memory
+constexpr long long FEW_PRODUCTS = 36LL << 20;
+
+// four codes (16 bits) -> magnitudes times two; mask: 0xff where the code is negative, 0x80 where not
+__device__ __forceinline__ unsigned fp4_magnitudes(unsigned c, unsigned& mask)
+{
+    // a selector's top bit spreads the chosen byte's sign (__byte_perm ignores that bit)
+    asm("prmt.b32 %0, %1, %1, %2;" : "=r"(mask) : "r"(0x80808080u), "r"(c));
+    return __byte_perm(0x03020100u, 0x0c080604u, c & 0x7777u);
+}
+// v * 2^e, e from -256 to 252
+__device__ __forceinline__ float scale_by(float v, int e)
+{
+    if ((unsigned) (e + 126) < 253u)
+        return v * __uint_as_float((unsigned) (e + 127) << 23);
+    const int h = e >> 1; // two factors that are floats
+    auto pow2 = [](int k) { return __uint_as_float(k > -127 ? (unsigned) (k + 127) << 23 : 0x00400000u >> (-127 - k)); };
+    return v * pow2(h) * pow2(e - h);
+}
+
+template <class T, int NT, int R>
+__global__ void __launch_bounds__(256) k_mx_times_few(const unsigned char* __restrict__ codesW, const unsigned char* __restrict__ scalesW,
+                                                      const unsigned char* __restrict__ codesX, const unsigned char* __restrict__ scalesX,
+                                                      const float* __restrict__ bias, T* __restrict__ y, long long ld, int O, int tokens, int blocks)
+{
+    extern __shared__ __align__(16) unsigned char few[];
+    uint4* x = reinterpret_cast<uint4*>(few);                 // [token][block][2]: 32 signed bytes
+    unsigned char* xs = few + (size_t) NT * blocks * 32;      // [token][block]
+    const int lane = threadIdx.x & 31;
+    const int unit = blockIdx.x * 8 + (threadIdx.x >> 5);
+    // two rows 32 apart: their scale bytes lie together
+    const int row0 = R == 2 ? unit / 64 * 128 + unit / 32 % 2 * 64 + unit % 32 : unit;
+    const long long chunks = (blocks + 3) / 4, pitch = blocks * 16LL;
+    const unsigned char *pw[R], *ps[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+    {
+        const int o = min(row0 + 32 * r, O - 1);
+        pw[r] = codesW + o * pitch;
+        ps[r] = scalesW + (o >> 7) * chunks * 512 + (o & 31) * 16 + (o >> 5 & 3) * 4;
+    }
+    uint4 wc[R];
+    unsigned wb[R];
+    auto fetch = [&](int b) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (b < blocks)
+            {
+                wc[r] = __ldcs(reinterpret_cast<const uint4*>(pw[r]) + b);
+                wb[r] = ps[r][(b >> 2) * 512LL + (b & 3)];
+            }
+    };
+    fetch(lane);
+    for (int i = threadIdx.x; i < NT * blocks; i += 256)
+    {
+        const int t = i / blocks, b = i - t * blocks;
+        if (t >= tokens)
+            break;
+        const uint4 c = reinterpret_cast<const uint4*>(codesX + t * pitch)[b];
+        xs[i] = scalesX[(b >> 2) * 512LL + t * 16 + (b & 3)];
+        unsigned v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+        {
+            const unsigned w = (&c.x)[q >> 1];
+            unsigned mask;
+            const unsigned mag = fp4_magnitudes(q & 1 ? w >> 16 : w & 0xffffu, mask);
+            v[q] = __vsub4(mag, 2u * (mag & mask));
+        }
+        x[2 * i] = make_uint4(v[0], v[1], v[2], v[3]);
+        x[2 * i + 1] = make_uint4(v[4], v[5], v[6], v[7]);
+    }
+    __syncthreads();
+    float sum[R][NT] = {};
+    for (int b = lane; b < blocks; b += 32)
+    {
+        uint4 w[R];
+        unsigned ws[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            w[r] = wc[r], ws[r] = wb[r];
+        fetch(b + 32);
+        int all[R][NT] = {}, negative[R][NT] = {};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+        {
+            uint4 xv[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                xv[t] = x[2 * (t * blocks + b) + h];
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                {
+                    const unsigned c = (&w[r].x)[2 * h + (q >> 1)];
+                    unsigned mask;
+                    const unsigned mag = fp4_magnitudes(q & 1 ? c >> 16 : c & 0xffffu, mask);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+                    {
+                        all[r][t] = __dp4a((int) mag, (int) (&xv[t].x)[q], all[r][t]);
+                        negative[r][t] = __dp4a((int) (mag & mask), (int) (&xv[t].x)[q], negative[r][t]);
+                    }
+                }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+        {
+            const unsigned xb = xs[t * blocks + b];
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+            {
+                const float v = scale_by((float) (all[r][t] - 2 * negative[r][t]), (int) (ws[r] + xb) - 256); // both operands are doubled
+                sum[r][t] += ws[r] == 255u || xb == 255u ? __uint_as_float(0x7fffffffu) : v;
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+        {
+#pragma unroll
+            for (int d = 16; d > 0; d /= 2)
+                sum[r][t] += __shfl_xor_sync(0xffffffffu, sum[r][t], d);
+            const int o = row0 + 32 * r;
+            if (lane == 0 && t < tokens && o < O)
+                put(y + t * ld + o, sum[r][t] + (bias ? bias[o] : 0.0f));
+        }
+}
+
+template <class T>
+static cudaError_t launch_times_few(cudaStream_t st, const void* wc, const void* ws, const void* xc, const void* xs, const float* bias, T* y, long long ld, long long O,
+                                    int tokens, long long K, int sms)
+{
+    const int blocks = (int) mx_blocks(K);
+    const bool two = O >= sms * 48LL; // a warp for every two rows still fills the SMs
+    const unsigned grid = (unsigned) (((two ? (O + 127) / 128 * 64 : O) + 7) / 8);
+    const auto launch = [&](auto kernel, int nt) {
+        kernel<<<grid, 256, nt * blocks * 33, st>>>((const unsigned char*) wc, (const unsigned char*) ws, (const unsigned char*) xc, (const unsigned char*) xs, bias, y, ld, (int) O,
+                                                    tokens, blocks);
+        return cudaGetLastError();
+    };
+    if (tokens == 1)
+        return two ? launch(k_mx_times_few<T, 1, 2>, 1) : launch(k_mx_times_few<T, 1, 1>, 1);
+    if (tokens == 2)
+        return two ? launch(k_mx_times_few<T, 2, 2>, 2) : launch(k_mx_times_few<T, 2, 1>, 2);
+    return two ? launch(k_mx_times_few<T, 4, 2>, 4) : launch(k_mx_times_few<T, 4, 1>, 4);
+}
+
 // ---- gradients --------------------------------------------------------------------------------------------------------------------
 
 struct GradArgs
@@ -1395,6 +1554,11 @@ int qagg_mx_times(void* stream, const void* w_codes, const void* w_scales, const
     rc = launch_cfg_for_current_device(&cfg);
     if (rc)
         return rc;
+    if (T <= FEW && K > 0 && (T == 3 ? 4 : T) * K <= FEW_VALUES && T * O * K <= FEW_PRODUCTS)
+    {
+        const auto few = [&](auto* p) { return launch_times_few((cudaStream_t) stream, w_codes, w_scales, x_codes, x_scales, bias, p, ld_y, O, (int) T, K, cfg.numSMs); };
+        return check_cuda(y_type == QAGG_F32 ? few((float*) y) : y_type == QAGG_F16 ? few((__half*) y) : few((__nv_bfloat16*) y), "4-bit product kernel launch");
+    }
     TimesArgs a = {};
     a.scaleW = (const unsigned char*) w_scales;
     a.scaleX = (const unsigned char*) x_scales;

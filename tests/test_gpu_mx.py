@@ -165,7 +165,9 @@ def test_offsets_beyond_32_bits(lib):
 
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("O,T,K,pad", [(128, 16, 256, 0), (1, 1, 1, 0), (128, 1, 32, 0), (129, 1, 2048, 0), (2048, 1, 2048, 0), (100, 3, 64, 5), (132, 17, 512, 0),
-                                       (512, 33, 363, 8), (300, 129, 429, 1), (256, 256, 1024, 0), (2048, 300, 429, 0), (520, 511, 96, 0), (1000, 1000, 1000, 0), (2200, 2500, 900, 0)])
+                                       (512, 33, 363, 8), (300, 129, 429, 1), (256, 256, 1024, 0), (2048, 300, 429, 0), (520, 511, 96, 0), (1000, 1000, 1000, 0), (2200, 2500, 900, 0), (2150, 2400, 900, 0), (5000, 1, 1100, 0),
+                                       (5000, 2, 429, 3), (5001, 4, 2048, 0), (77, 4, 5000, 0), (40, 5, 333, 0),
+                                       (33, 4, 8192, 0), (33, 4, 8193, 0), (20, 1, 40000, 0), (9300, 3, 200, 0), (9304, 4, 1024, 0)])
 def test_times(lib, O, T, K, pad, t):
     rng = np.random.default_rng(O + T + K)
     (wc, ws), w = packed(rng, O, K, mx_util.FP4, 0.05)
@@ -190,7 +192,7 @@ def test_times_without_inputs_is_the_bias(lib):
     assert not y.any()
 
 
-@pytest.mark.parametrize("T", [3, 200])
+@pytest.mark.parametrize("T", [3, 7, 200])
 def test_times_scales_and_bad_blocks(lib, T):
     """Each block's scale goes with its own 32 values; a NaN block spoils its row of results and no other."""
     O, K = 130, 300
@@ -204,6 +206,27 @@ def test_times_scales_and_bad_blocks(lib, T):
     y = torch.zeros(T, O, device=DEV)
     lib.mx_times(wc.data_ptr(), ws.data_ptr(), xc.data_ptr(), xs.data_ptr(), 0, y.data_ptr(), lib.F32, O, O, T, K, stream())
     check(y, x @ w.T, np.abs(x) @ np.abs(w).T, K / 16, "f32", "times with scales")
+
+
+@pytest.mark.parametrize("T", [2, 20])
+def test_times_at_the_ends_of_the_range(lib, T):
+    """Scales whose product is in range though each is far from it, and sums that leave the range."""
+    O, K = 40, 64
+    rng = np.random.default_rng(6)
+    xw = rng.standard_normal((O, K)).clip(-1.4, 1.4) * np.exp2(np.linspace(-120, 120, O).round())[:, None]
+    xx = np.stack([rng.standard_normal(K).clip(-1.4, 1.4) * 2.0 ** (-100 if t % 2 else 60) for t in range(T)])
+    (wc, ws), (xc, xs) = to_dev(*mx_util.pack(xw, 4)), to_dev(*mx_util.pack(xx, 4))
+    w, x = mx_util.values(xw, 4), mx_util.values(xx, 4)
+    y = torch.zeros(T, O, device=DEV)
+    lib.mx_times(wc.data_ptr(), ws.data_ptr(), xc.data_ptr(), xs.data_ptr(), 0, y.data_ptr(), lib.F32, O, O, T, K, stream())
+    got, want, mags = y.double().cpu().numpy(), x @ w.T, np.abs(x) @ np.abs(w).T
+    top = 3.4028235e38
+    # results below the smallest normal may be flushed; where the terms leave the range a sum of fp32 numbers is infinite, or NaN (two
+    # terms of opposite signs)
+    ok = np.abs(got - want) <= 10 * 2.0 ** -22 * mags + 2.0 ** -126
+    over = mags > top / 2
+    assert (ok | over).all()
+    assert (~np.isfinite(got) | ok)[over].all()
 
 
 # ---- gradients ----------------------------------------------------------------------------------------------------------------
