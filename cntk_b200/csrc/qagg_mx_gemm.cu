@@ -1045,7 +1045,7 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
 
     if (warp < 4)
     {
-        registers_down<G::regsMisc>();
+        set_registers<G::regsMisc, G::regsLaunch>();
         if (warp == 0 && elect_one())
         {
             Ring ring;
@@ -1123,7 +1123,7 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
     }
     else if (warp < G::firstResult)
     {
-        registers_down<G::regsExpand>();
+        set_registers<G::regsExpand, G::regsLaunch>();
         // Expand: lanes 32 * quad .. of the tile are one block of the packed matrix, so a warp has one scale per contraction value.
         // The codes lie [contraction value][row]; ldmatrix transposes 16 x 16 bytes of them into the order in which a 16 x 256-bit
         // store to tensor memory takes pairs of contraction values.  With fp4 that puts row 16 h + 2 b + o of the block on lane
@@ -1224,7 +1224,7 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
     }
     else if (warp < G::firstLoad)
     {
-        registers_up<G::regsResult>();
+        set_registers<G::regsResult, G::regsLaunch>();
         const int rw = warp - G::firstResult, quad = rw & 3, half = rw >> 2;
         {
             const int cols = bn / G::result;
@@ -1267,7 +1267,7 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
     else if constexpr (DENSE > 0)
     {
         // Two steps' values are on their way (behind the fence, which would wait for them) while an earlier one is split and stored.
-        registers_down<G::regsLoad>();
+        set_registers<G::regsLoad, G::regsLaunch>();
         unsigned char* mine = stage0 + (unit >> 3) * 128 + (((unit & 7) ^ (unit >> 3 & 7)) << 4);
         Ring ring;
         long long done = 0;

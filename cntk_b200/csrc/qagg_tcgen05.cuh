@@ -142,16 +142,15 @@ __device__ __forceinline__ void ldmatrix_trans_b8(unsigned addr, unsigned (&r)[4
 {
     asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-// registers per thread of this warp's group of four warps, whose warps all get here
-template <int N>
-__device__ __forceinline__ void registers_up()
+// Registers per thread of this warp's group of four warps, whose warps all get here, from LAUNCHED to N.  (A decrease to more than a warp
+// has is an illegal instruction.)
+template <int N, int LAUNCHED>
+__device__ __forceinline__ void set_registers()
 {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void registers_down()
-{
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+    if constexpr (N > LAUNCHED)
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+    else if constexpr (N < LAUNCHED)
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 __device__ __forceinline__ void tmem_store_wait()
 {
