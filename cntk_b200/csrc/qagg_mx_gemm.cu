@@ -35,9 +35,10 @@ __device__ unsigned g_mxStatus;
 constexpr unsigned TMEM_COLS = 512; // accumulators first; behind them block scales or expanded operands
 constexpr int MAX_STAGES = 8;
 constexpr int GEMM_SMEM_MAX = 224 * 1024; // dynamic; barriers and scales take a little more
-// More than half of an SM's shared memory, always: a second CTA on the SM would wait for tensor memory (all columns are taken),
-// and CTAs of two clusters that each wait for the other's tensor memory would never meet at their cluster barriers.
-constexpr int GEMM_SMEM_MIN = 118 * 1024;
+// Nearly all of an SM's shared memory, always: a second CTA on the SM, of these kernels or of any other that uses tensor memory, would
+// wait for the columns this one holds, and CTAs of two clusters that each wait for the other's would never meet at their cluster
+// barriers.
+constexpr int GEMM_SMEM_MIN = 200 * 1024;
 // tensor-core instructions in a row on one accumulator: their truncation stays near 5e-7 of the sum
 constexpr int CHAIN = 32, CHAIN_16BIT = 1024;
 

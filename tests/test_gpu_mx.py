@@ -453,3 +453,191 @@ def test_slope_against_differences(lib, act):
     lib.mx_act_backward(dx.data_ptr(), lib.F32, 32, codes.data_ptr(), scales.data_ptr(), act, dx.data_ptr(), 32, 32, 8, stream())
     # third derivatives are below 4: h^2 / 6 * 4; the forward's rounding of values below 5: 12 * 2^-24 * 5 / h
     assert np.abs(dx.double().cpu().numpy() - diff).max() <= h * h * 4 / 6 + 12 * 2.0 ** -24 * 5 / h
+
+
+# ---- together -----------------------------------------------------------------------------------------------------------------
+
+
+def quantized(lib, d, m, n, ld, t, fmt, transpose=False):
+    pm, pn = (n, m) if transpose else (m, n)
+    codes = torch.empty(lib.mx_code_bytes(pm, pn, fmt), dtype=torch.uint8, device=DEV)
+    scales = torch.empty(lib.mx_scale_bytes(pm, pn), dtype=torch.uint8, device=DEV)
+    lib.mx_quantize(d.data_ptr(), code(lib, t), ld, codes.data_ptr(), scales.data_ptr(), m, n, fmt, transpose, stream())
+    return codes, scales
+
+
+class TwoLayers:
+    """y = W2 gelu(W1 x + b1): forward with 4-bit products, x and the hidden layer's input kept in 8 bits, the hidden layer's output in
+    its 4-bit form; backward from what was kept; the weight gradients go through the 1-bit aggregation step."""
+
+    def __init__(self, lib, I, H, O, T, t):
+        self.lib, self.I, self.H, self.O, self.T, self.t = lib, I, H, O, T, t
+        new = lambda n, m, ty=t: torch.zeros(n, m, dtype=TYPES[ty], device=DEV)
+        self.x, self.dy = new(T, I), new(T, O)
+        self.w1, self.w2, self.b1 = new(I, H, "f32"), new(H, O, "f32"), torch.zeros(H, device=DEV)
+        self.z, self.h, self.y, self.dh, self.dz = new(T, H), new(T, H), new(T, O), new(T, H), new(T, H)
+        flat = torch.zeros(I * H + H * O, device=DEV)
+        self.dw1, self.dw2 = flat[: I * H].view(I, H), flat[I * H:].view(H, O)
+
+    def run(self):
+        lib, I, H, O, T, t = self.lib, self.I, self.H, self.O, self.T, code(self.lib, self.t)
+        p = lambda pair: (pair[0].data_ptr(), pair[1].data_ptr())
+        self.w1q, self.w2q = quantized(lib, self.w1, H, I, H, "f32", lib.MXFP4, True), quantized(lib, self.w2, O, H, O, "f32", lib.MXFP4, True)
+        self.xq, self.x8 = quantized(lib, self.x, I, T, I, self.t, lib.MXFP4), quantized(lib, self.x, I, T, I, self.t, lib.MXINT8)
+        lib.mx_times(*p(self.w1q), *p(self.xq), self.b1.data_ptr(), self.z.data_ptr(), t, H, H, T, I, stream())
+        self.z8 = [torch.empty(lib.mx_code_bytes(H, T, 8), dtype=torch.uint8, device=DEV), torch.empty(lib.mx_scale_bytes(H, T), dtype=torch.uint8, device=DEV)]
+        lib.mx_act_forward(self.z.data_ptr(), t, H, lib.ACT_GELU, self.h.data_ptr(), H, *p(self.z8), H, T, stream())
+        self.hq = quantized(lib, self.h, H, T, H, self.t, lib.MXFP4)
+        lib.mx_times(*p(self.w2q), *p(self.hq), 0, self.y.data_ptr(), t, O, O, T, H, stream())
+        lib.mx_weight_grad(self.dy.data_ptr(), t, O, *p(self.hq), lib.MXFP4, self.dw2.data_ptr(), O, H, T, False, stream())
+        lib.mx_input_grad(self.dy.data_ptr(), t, O, *p(self.w2q), lib.MXFP4, self.dh.data_ptr(), t, H, O, H, T, stream())
+        lib.mx_act_backward(self.dh.data_ptr(), t, H, *p(self.z8), lib.ACT_GELU, self.dz.data_ptr(), H, H, T, stream())
+        lib.mx_weight_grad(self.dz.data_ptr(), t, H, *p(self.x8), lib.MXINT8, self.dw1.data_ptr(), H, I, T, False, stream())
+
+    def fill(self, seed):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        for a, s in ((self.x, 1.0), (self.dy, 0.1), (self.w1, 0.05), (self.w2, 0.05), (self.b1, 0.1)):
+            a.copy_(torch.empty(a.shape, device=DEV).normal_(0.0, s, generator=g))
+
+    def check(self):
+        """Each step against the formula at what the step before it left."""
+        v = lambda a: a.double().cpu().numpy()
+        q = lambda a, fmt: mx_util.values(v(a), fmt)
+        w1, w2 = q(self.w1.t(), 4), q(self.w2.t(), 4)  # [outputs, inputs]
+        x4, x8, h4, z8 = q(self.x, 4), q(self.x, 8), q(self.h, 4), q(self.z, 8)
+        I, H, O, T, t = self.I, self.H, self.O, self.T, self.t
+        planes = {"bf16": 1, "f16": 2, "f32": 3}[t]
+        check(self.z, x4 @ w1.T + v(self.b1), np.abs(x4) @ np.abs(w1).T + 1, I / 16, t, "z")
+        check(self.y, h4 @ w2.T, np.abs(h4) @ np.abs(w2).T, H / 16, t, "y")
+        dy, dh, dz = v(self.dy), v(self.dh), v(self.dz)
+        check(self.dw2, h4.T @ dy, np.abs(h4).T @ np.abs(dy), planes * T / 16, "f32", "dw2")
+        check(self.dh, dy @ w2, np.abs(dy) @ np.abs(w2), planes * O / 16, t, "dh")
+        eps = torch.finfo(TYPES[t]).eps
+        want = f64(v(self.z), 3)[0]
+        assert (np.abs(v(self.h) - want) <= 12 * 2.0 ** -24 * (np.abs(v(self.z)) + 1) + eps / 2 * np.abs(want) + 2.0 ** -25).all()
+        want = dh * f64(z8, 3)[1]
+        assert (np.abs(dz - want) <= 12 * 2.0 ** -24 * np.abs(dh) * (np.abs(z8) + 1) + eps / 2 * np.abs(want) + 2.0 ** -25).all()
+        check(self.dw1, x8.T @ dz, np.abs(x8).T @ np.abs(dz), planes * T / 16, "f32", "dw1")
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("I,H,O,T", [(363, 512, 132, 256), (429, 264, 100, 77), (64, 32, 16, 1)])
+def test_a_training_step(lib, I, H, O, T, t):
+    """Forward, backward, aggregation: the gradients that come out are what the aggregation step takes and quantizes."""
+    net = TwoLayers(lib, I, H, O, T, t)
+    net.fill(7)
+    net.run()
+    lib.mx_check(stream())
+    net.check()
+    grads = [net.dw1.clone(), net.dw2.clone()]
+    shapes = [(H, I), (O, H)]
+    comm = lib.Comm.create(None, 0, 1, 0)
+    agg = lib.Aggregator(comm, shapes, 1)
+    agg.step([net.dw1.data_ptr(), net.dw2.data_ptr()], stream())
+    torch.cuda.synchronize()
+    for (m, n), g, d in zip(shapes, grads, (net.dw1, net.dw2)):
+        residual, out = torch.zeros_like(g), torch.zeros_like(g)
+        packed = torch.zeros(lib.packed_bytes(m, n, 1), dtype=torch.uint8, device=DEV)
+        lib.quantize(g.data_ptr(), residual.data_ptr(), residual.data_ptr(), packed.data_ptr(), m, n, 1, True, stream())
+        lib.unquantize(packed.data_ptr(), out.data_ptr(), m, n, 1, False, stream())
+        torch.cuda.synchronize()
+        assert torch.equal(out, d)
+    agg.destroy()
+    comm.destroy()
+
+
+def test_a_captured_step_replayed(lib):
+    """One graph, three replays over other inputs in the same buffers, an eager step on another stream between them."""
+    net, other = TwoLayers(lib, 200, 264, 144, 300, "bf16"), TwoLayers(lib, 200, 264, 144, 300, "bf16")
+    net.fill(1)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        net.run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        net.run()
+    for seed in (2, 3, 4):
+        net.fill(seed)
+        other.fill(seed + 10)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graph.replay()
+        other.run()
+        torch.cuda.synchronize()
+        net.check()
+        other.check()
+
+
+def test_products_on_two_streams(lib):
+    """Kernels that each want whole SMs, and clusters of them, on two streams at once: the same bits as one after the other."""
+    rng = np.random.default_rng(4)
+    work = []
+    for O, I, T, t in ((2048, 1100, 2100, "bf16"), (132, 512, 256, "f32"), (700, 300, 4096, "bf16"), (512, 363, 64, "f16")):
+        _, d, _ = dense(rng, T, O, t, 0, 0, 1e-2)
+        (xc, xs), _ = packed(rng, T, I, 8)
+        (wc, ws), _ = packed(rng, O, I, 4, 0.05)
+        (x4c, x4s), _ = packed(rng, T, I, 4)
+        out = [torch.zeros(I, O, device=DEV), torch.zeros(T, I, dtype=TYPES[t], device=DEV), torch.zeros(T, O, device=DEV)]
+
+        def run(O=O, I=I, T=T, t=t, d=d, xc=xc, xs=xs, wc=wc, ws=ws, x4c=x4c, x4s=x4s, out=out):
+            lib.mx_weight_grad(d.data_ptr(), code(lib, t), O, xc.data_ptr(), xs.data_ptr(), 8, out[0].data_ptr(), O, I, T, False, stream())
+            lib.mx_input_grad(d.data_ptr(), code(lib, t), O, wc.data_ptr(), ws.data_ptr(), 4, out[1].data_ptr(), code(lib, t), I, O, I, T, stream())
+            lib.mx_times(wc.data_ptr(), ws.data_ptr(), x4c.data_ptr(), x4s.data_ptr(), 0, out[2].data_ptr(), lib.F32, O, O, T, I, stream())
+
+        work.append((run, out))
+    for run, _ in work:
+        run()
+    torch.cuda.synchronize()
+    want = [[o.clone() for o in out] for _, out in work]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for turn in range(6):
+        for _, out in work:
+            for o in out:
+                o.zero_()
+        torch.cuda.synchronize()
+        for k, (run, _) in enumerate(work):
+            with torch.cuda.stream(streams[(k + turn) % 2]):
+                run()
+        lib.mx_check(streams[0].cuda_stream)
+        torch.cuda.synchronize()
+        for (_, out), w in zip(work, want):
+            assert all(torch.equal(a, b) for a, b in zip(out, w))
+
+
+def test_products_with_columns_far_apart(lib):
+    """Columns 2^31 values apart: the third begins beyond 2^32."""
+    O, I, T, ld = 64, 40, 3, (1 << 31) + 64
+    rng = np.random.default_rng(9)
+    big = torch.zeros(2 * ld + 128, dtype=torch.bfloat16, device=DEV)
+    dy = torch.from_numpy(rng.standard_normal((T, O))).to(torch.bfloat16)
+    (xc, xs), x = packed(rng, T, I, 8)
+    (wc, ws), w = packed(rng, O, I, 4)
+    v = dy.double().numpy()
+    for off in (0, 1):  # the copy engine's way, and the loaders'
+        for j in range(T):
+            big[off + j * ld:off + j * ld + O] = dy[j].to(DEV)
+        at = big.data_ptr() + 2 * off
+        dw = torch.zeros(I, O, device=DEV)
+        lib.mx_weight_grad(at, lib.BF16, ld, xc.data_ptr(), xs.data_ptr(), 8, dw.data_ptr(), O, I, T, False, stream())
+        check(dw, x.T @ v, np.abs(x).T @ np.abs(v), 1, "f32", "weight gradient")
+        dx = torch.zeros(T, I, device=DEV)
+        lib.mx_input_grad(at, lib.BF16, ld, wc.data_ptr(), ws.data_ptr(), 4, dx.data_ptr(), lib.F32, I, O, I, T, stream())
+        check(dx, v @ w, np.abs(v) @ np.abs(w), O / 16, "f32", "input gradient")
+    near = dy.to(DEV)
+    lib.mx_input_grad(near.data_ptr(), lib.BF16, O, wc.data_ptr(), ws.data_ptr(), 4, big.data_ptr(), lib.BF16, ld, O, I, T, stream())
+    check(torch.stack([big[j * ld:j * ld + I] for j in range(T)]), v @ w, np.abs(v) @ np.abs(w), O / 16, "bf16", "input gradient far apart")
+
+
+@pytest.mark.parametrize("O,T", [(2200, 2500), (300, 40)])
+def test_large_products_of_nothing(lib, O, T):
+    bias = torch.arange(O, dtype=torch.float32, device=DEV)
+    y = torch.full((T, O), GUARD, device=DEV)
+    lib.mx_times(0, 0, 0, 0, bias.data_ptr(), y.data_ptr(), lib.F32, O, O, T, 0, stream())
+    assert torch.equal(y, bias.expand(T, O))
+    y.fill_(GUARD)
+    lib.mx_weight_grad(0, lib.BF16, O, 0, 0, 8, y.data_ptr(), O, T, 0, False, stream())
+    assert not y.any()
+    y.fill_(GUARD)
+    lib.mx_input_grad(0, lib.BF16, 0, 0, 0, 4, y.data_ptr(), lib.F32, O, 0, O, T, stream())
+    assert not y.any()
