@@ -39,8 +39,9 @@ constexpr int GEMM_SMEM_MAX = 224 * 1024; // dynamic; barriers and scales take a
 // wait for the columns this one holds, and CTAs of two clusters that each wait for the other's would never meet at their cluster
 // barriers.
 constexpr int GEMM_SMEM_MIN = 200 * 1024;
-// tensor-core instructions in a row on one accumulator: their truncation stays near 5e-7 of the sum
-constexpr int CHAIN = 32, CHAIN_16BIT = 1024;
+// Tensor-core instructions in a row on one accumulator.  After 32 the sums are within 3e-7; with a single accumulator, where every
+// chain costs its hand-over, 64 are taken: within 6e-7, as a sum in plain fp32 is.
+constexpr int CHAIN = 32, CHAIN_SINGLE = 64, CHAIN_16BIT = 1024;
 
 struct GemmBars
 {
@@ -405,7 +406,7 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
     const int resultWarps = bn > 128 ? 8 : 4;
     const int bufs = bn > 128 ? 1 : 2; // accumulators, 128 columns apart
     constexpr unsigned SIDE = 256;     // block scales: 24 columns a stage
-    constexpr int CHAIN_STEPS = (sizeof(T) == 4 ? CHAIN : CHAIN_16BIT) / 4;
+    constexpr int CHAIN_STEPS = (sizeof(T) != 4 ? CHAIN_16BIT : ACC == 128 ? CHAIN_SINGLE : CHAIN) / 4;
 
     // The copying thread's time per step counts: what depends on the tile alone is worked out once per tile.
     struct Source
@@ -918,7 +919,7 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
     using G = GradGroups<(DENSE > 0), PAIR>;
     static_assert(!(PAIR && DENSE), "pairs bring dy through the copy engine");
     constexpr int NP = DENSE ? DENSE : 1;
-    constexpr int CHAIN_STEPS = (sizeof(TO) == 4 ? CHAIN : CHAIN_16BIT) / 4 / NP;
+    constexpr int CHAIN_STEPS = (sizeof(TO) != 4 ? CHAIN_16BIT : PAIR ? CHAIN_SINGLE : CHAIN) / 4 / NP;
     constexpr int WIDEST = G::widest, SLOTS = G::slots, BUFS = G::accumulators;
     extern __shared__ unsigned char dyn[];
     __shared__ GemmBars bars;
