@@ -2,9 +2,10 @@
 // that keep their input in 8 bits for the backward pass.  The form is described in qagg_mx.cuh.
 //
 // All kernels here move each value once and are bound by HBM.  One CTA takes one scale tile: 128 packed columns x 4 blocks.
-// A thread takes 16 bytes of dense values at a time (eight of a 16-bit type, four fp32: whole warps then read and write whole lines),
-// so four or eight threads share a block, its largest magnitude takes two or three shuffles, and the tile's 512 scale bytes are
-// collected in shared memory and leave as full lines.
+// A thread takes 32 bytes of dense values at a time, with one 256-bit access where they are aligned (sixteen values of a 16-bit type,
+// eight fp32): what a block costs, the largest magnitude, the scale, the addresses, is shared by more values than with 16 bytes, and a
+// warp still reads and writes whole sectors.  Two or four threads share a block; the tile's 512 scale bytes are collected in shared
+// memory and leave as full lines.
 #include "qagg_mx.cuh"
 
 #include <algorithm>
@@ -18,12 +19,19 @@ constexpr int MX_TILE = 128; // rows and columns of a tile
 template <class T, bool ACT = false>
 struct Shape // of the threads over a tile; ACT: with a function's arithmetic, which needs the registers
 {
-    static constexpr int V = 16 / sizeof(T);             // values per thread and turn
-    static constexpr int LANES = MX_TILE / V;            // threads per column
-    static constexpr int COLS = MXT / LANES;             // columns per pass
+    static constexpr int V = 32 / sizeof(T);  // values per thread and turn
+    static constexpr int LANES = MX_TILE / V; // threads per column
+    static constexpr int COLS = MXT / LANES;  // columns per pass
     static constexpr int PASSES = MX_TILE / COLS;
-    static constexpr int FLIGHT = ACT ? 2 : 8; // passes whose loads are in flight together
+    static constexpr int FLIGHT = ACT ? 1 : 4; // passes whose loads are in flight together
+    static constexpr int PARTS = MX_BLOCK / V; // threads per block
 };
+struct Raw32
+{
+    uint4 a, b;
+};
+// how a matrix may be accessed: 32 bytes a time, 16, or value by value
+constexpr int VEC32 = 2, VEC16 = 1;
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
@@ -37,14 +45,28 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// 16 bytes of values: n of them exist, the others read as zero.  vec: the address is 16-byte aligned.
+// 32 bytes of values: n of them exist, the others read as zero.  Dense values pass once: first to leave L2, so that codes and scales, which
+// the next kernel wants, stay (2048 x 16384 to int8 and back: 50.5 us with plain streaming accesses, 44.8 so).
 template <class T>
-__device__ __forceinline__ uint4 load16(const T* p, int n, bool vec)
+__device__ __forceinline__ Raw32 load32(const T* p, int n, int vec)
 {
     constexpr int V = Shape<T>::V;
-    uint4 r = make_uint4(0, 0, 0, 0);
+    Raw32 r;
+    if (vec == VEC32 && n == V)
+    {
+        asm volatile("ld.global.L1::no_allocate.L2::evict_first.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(r.a.x), "=r"(r.a.y), "=r"(r.a.z), "=r"(r.a.w), "=r"(r.b.x), "=r"(r.b.y), "=r"(r.b.z), "=r"(r.b.w)
+                     : "l"(p));
+        return r;
+    }
+    r.a = r.b = make_uint4(0, 0, 0, 0);
     if (vec && n == V)
-        return __ldcs(reinterpret_cast<const uint4*>(p));
+    {
+        const uint4* q = reinterpret_cast<const uint4*>(p);
+        r.a = __ldcs(q);
+        r.b = __ldcs(q + 1);
+        return r;
+    }
     T* e = reinterpret_cast<T*>(&r);
 #pragma unroll
     for (int i = 0; i < V; ++i)
@@ -53,7 +75,7 @@ __device__ __forceinline__ uint4 load16(const T* p, int n, bool vec)
     return r;
 }
 template <class T>
-__device__ __forceinline__ void unpack16(const uint4& r, float (&v)[Shape<T>::V])
+__device__ __forceinline__ void unpack32(const Raw32& r, float (&v)[Shape<T>::V])
 {
     const T* e = reinterpret_cast<const T*>(&r);
 #pragma unroll
@@ -61,16 +83,24 @@ __device__ __forceinline__ void unpack16(const uint4& r, float (&v)[Shape<T>::V]
         v[i] = to_float(e[i]);
 }
 template <class T>
-__device__ __forceinline__ void store16(T* p, const float (&v)[Shape<T>::V], int n, bool vec)
+__device__ __forceinline__ void store32(T* p, const float (&v)[Shape<T>::V], int n, int vec)
 {
     constexpr int V = Shape<T>::V;
-    uint4 r;
+    Raw32 r;
     T* e = reinterpret_cast<T*>(&r);
 #pragma unroll
     for (int i = 0; i < V; ++i)
         e[i] = from_float<T>(v[i]);
-    if (vec && n == V)
-        __stcs(reinterpret_cast<uint4*>(p), r);
+    if (vec == VEC32 && n == V)
+        asm volatile("st.global.L1::no_allocate.L2::evict_first.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r.a.x), "r"(r.a.y), "r"(r.a.z), "r"(r.a.w), "r"(r.b.x), "r"(r.b.y),
+                     "r"(r.b.z), "r"(r.b.w)
+                     : "memory");
+    else if (vec && n == V)
+    {
+        uint4* q = reinterpret_cast<uint4*>(p);
+        __stcs(q, r.a);
+        __stcs(q + 1, r.b);
+    }
     else
     {
 #pragma unroll
@@ -79,6 +109,54 @@ __device__ __forceinline__ void store16(T* p, const float (&v)[Shape<T>::V], int
                 p[i] = e[i];
     }
 }
+
+// Matrices whose columns are not 16-byte aligned: a warp's columns of one pass (32 bytes a lane) are read and written value by value,
+// neighbouring lanes neighbouring values, and change hands in the warp's kilobyte of shared memory.
+template <class T>
+struct Exchange
+{
+    static constexpr int V = Shape<T>::V;
+    T v[V]; // value 32 j + lane of the warp's columns, 128 rows each
+    __device__ __forceinline__ void fetch(const T* first, long long ld, int rows, int cols)
+    {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+        {
+            const int at = j * 32 + lane, c = at / MX_TILE, r = at % MX_TILE;
+            v[j] = c < cols && r < rows ? first[c * ld + r] : from_float<T>(0.0f);
+        }
+    }
+    __device__ __forceinline__ Raw32 take(T* room) const // what load32 gives
+    {
+        const int lane = threadIdx.x & 31;
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            room[j * 32 + lane] = v[j];
+        __syncwarp();
+        return reinterpret_cast<const Raw32*>(room)[lane];
+    }
+    static __device__ __forceinline__ void put(T* room, const float (&value)[V], T* first, long long ld, int rows, int cols)
+    {
+        const int lane = threadIdx.x & 31;
+        Raw32 r;
+        T* e = reinterpret_cast<T*>(&r);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            e[i] = from_float<T>(value[i]);
+        __syncwarp();
+        reinterpret_cast<Raw32*>(room)[lane] = r;
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+        {
+            const int at = j * 32 + lane, c = at / MX_TILE, r_ = at % MX_TILE;
+            if (c < cols && r_ < rows)
+                first[c * ld + r_] = room[at];
+        }
+    }
+};
 
 // ---- elements ---------------------------------------------------------------------------------------------------------------
 
@@ -283,14 +361,17 @@ __device__ __forceinline__ float act_slope(float x)
     }
 }
 
-// Bit pattern, as a float's, of the largest magnitude of a thread's 16 bytes; 16-bit types two at a time.
+// Bit pattern, as a float's, of the largest magnitude of a thread's 32 bytes; 16-bit types two at a time.
 template <class T>
-__device__ __forceinline__ unsigned largest16(const uint4& r)
+__device__ __forceinline__ unsigned largest32(const Raw32& raw)
 {
+    const uint4 r = raw.a, q = raw.b;
     if constexpr (sizeof(T) == 4)
-        return max(max(r.x & 0x7fffffffu, r.y & 0x7fffffffu), max(r.z & 0x7fffffffu, r.w & 0x7fffffffu));
+        return max(max(max(r.x & 0x7fffffffu, r.y & 0x7fffffffu), max(r.z & 0x7fffffffu, r.w & 0x7fffffffu)),
+                   max(max(q.x & 0x7fffffffu, q.y & 0x7fffffffu), max(q.z & 0x7fffffffu, q.w & 0x7fffffffu)));
     else
-        return __vmaxu2(__vmaxu2(r.x & 0x7fff7fffu, r.y & 0x7fff7fffu), __vmaxu2(r.z & 0x7fff7fffu, r.w & 0x7fff7fffu));
+        return __vmaxu2(__vmaxu2(__vmaxu2(r.x & 0x7fff7fffu, r.y & 0x7fff7fffu), __vmaxu2(r.z & 0x7fff7fffu, r.w & 0x7fff7fffu)),
+                        __vmaxu2(__vmaxu2(q.x & 0x7fff7fffu, q.y & 0x7fff7fffu), __vmaxu2(q.z & 0x7fff7fffu, q.w & 0x7fff7fffu)));
 }
 template <class T, int THREADS>
 __device__ __forceinline__ unsigned largest_of_block(unsigned top)
@@ -332,49 +413,79 @@ __global__ void __launch_bounds__(MXT, (ACT >= 0 ? 5 : 4)) k_mx_quantize(const T
     T* py = y + (col0 + c0) * ldy + row;
     unsigned char* pc = codes + (col0 + c0) * pitch + (FMT == QAGG_MXFP4 ? row / 2 : row);
     const int cols = (int) (N - col0 - c0 < MX_TILE ? N - col0 - c0 : MX_TILE); // columns from this thread's first on
-#pragma unroll 1
-    for (int h = 0; h < MX_TILE; h += S::FLIGHT * S::COLS)
-    {
-        uint4 raw[S::FLIGHT];
-#pragma unroll
-        for (int p = 0; p < S::FLIGHT; ++p)
-            raw[p] = load16(px + p * S::COLS * ldx, h + p * S::COLS < cols ? n : 0, vecX);
-#pragma unroll
-        for (int p = 0; p < S::FLIGHT; ++p)
+    // value by value: the warp's rows and columns, from its first column on
+    __shared__ __align__(32) unsigned char rooms[MXT / 32][1024];
+    T* room = reinterpret_cast<T*>(rooms[tid >> 5]);
+    const int lane0 = (tid & 31) / S::LANES;
+    const int rows = (int) (M - row0 < MX_TILE ? M - row0 : MX_TILE);
+    const auto one = [&](const Raw32& raw, int c, unsigned char* at, T* yAt) { // c: column of the tile, from this thread's first
+        const BlockEncoder<FMT> enc(largest_of_block<T, S::PARTS>(largest32<T>(raw)));
+        float v[S::V];
+        unpack32<T>(raw, v);
+        if (c < cols && block)
         {
-            const int c = h + p * S::COLS; // from this thread's first column
-            float v[S::V];
-            unpack16<T>(raw[p], v);
-            const BlockEncoder<FMT> enc(largest_of_block<T, MX_BLOCK / S::V>(largest16<T>(raw[p])));
-            if (c < cols && block)
-            {
-                unsigned w[2];
+            unsigned w[S::V / 4];
 #pragma unroll
-                for (int q = 0; q < S::V / 4; ++q)
-                    w[q] = enc.encode4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-                unsigned char* at = pc + p * S::COLS * pitch;
-                if constexpr (FMT == QAGG_MXFP4 && S::V == 4)
-                    *reinterpret_cast<unsigned short*>(at) = (unsigned short) w[0];
-                else if constexpr (FMT == QAGG_MXFP4)
-                    *reinterpret_cast<unsigned*>(at) = w[0] | w[1] << 16;
-                else if constexpr (S::V == 4)
-                    *reinterpret_cast<unsigned*>(at) = w[0];
-                else
-                    *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
-                if (seg % (MX_BLOCK / S::V) == 0)
-                    tile[((c0 + c) & 31) * 16 + ((c0 + c) >> 5) * 4 + b] = (unsigned char) enc.byte;
-                if constexpr (ACT >= 0)
-                {
-#pragma unroll
-                    for (int i = 0; i < S::V; ++i)
-                        v[i] = act_value<ACT, T>(v[i]);
-                    store16(py + p * S::COLS * ldy, v, n, vecY);
-                }
-            }
+            for (int q = 0; q < S::V / 4; ++q)
+                w[q] = enc.encode4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+            if constexpr (FMT == QAGG_MXFP4 && S::V == 8)
+                *reinterpret_cast<unsigned*>(at) = w[0] | w[1] << 16;
+            else if constexpr (FMT == QAGG_MXFP4)
+                *reinterpret_cast<uint2*>(at) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+            else if constexpr (S::V == 8)
+                *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
+            else
+                *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (seg % S::PARTS == 0)
+                tile[((c0 + c) & 31) * 16 + ((c0 + c) >> 5) * 4 + b] = (unsigned char) enc.byte;
         }
-        px += S::FLIGHT * S::COLS * ldx;
-        py += S::FLIGHT * S::COLS * ldy;
-        pc += S::FLIGHT * S::COLS * pitch;
+        if constexpr (ACT >= 0)
+        {
+#pragma unroll
+            for (int i = 0; i < S::V; ++i)
+                v[i] = act_value<ACT, T>(v[i]);
+            if (vecY)
+            {
+                if (c < cols && block)
+                    store32(yAt, v, n, vecY);
+            }
+            else
+                Exchange<T>::put(room, v, yAt - seg * S::V - lane0 * ldy, ldy, rows, cols + lane0 - c);
+        }
+    };
+    if (vecX)
+    {
+#pragma unroll 1
+        for (int h = 0; h < MX_TILE; h += S::FLIGHT * S::COLS)
+        {
+            Raw32 raw[S::FLIGHT];
+#pragma unroll
+            for (int p = 0; p < S::FLIGHT; ++p)
+                raw[p] = load32(px + p * S::COLS * ldx, h + p * S::COLS < cols ? n : 0, vecX);
+#pragma unroll
+            for (int p = 0; p < S::FLIGHT; ++p)
+                one(raw[p], h + p * S::COLS, pc + p * S::COLS * pitch, py + p * S::COLS * ldy);
+            px += S::FLIGHT * S::COLS * ldx;
+            py += S::FLIGHT * S::COLS * ldy;
+            pc += S::FLIGHT * S::COLS * pitch;
+        }
+    }
+    else
+    {
+        px -= seg * S::V + lane0 * ldx; // the warp's first
+        Exchange<T> next;
+        next.fetch(px, ldx, rows, cols + lane0);
+#pragma unroll 1
+        for (int h = 0; h < MX_TILE; h += S::COLS)
+        {
+            const Raw32 raw = next.take(room);
+            px += S::COLS * ldx;
+            if (h + S::COLS < MX_TILE)
+                next.fetch(px, ldx, rows, cols + lane0 - h - S::COLS);
+            one(raw, h, pc, py);
+            py += S::COLS * ldy;
+            pc += S::COLS * pitch;
+        }
     }
     __syncthreads();
     if (tid < 32)
@@ -404,11 +515,26 @@ __global__ void __launch_bounds__(MXT) k_mx_quantize_t(const T* __restrict__ x, 
         const int seg = tid % S::LANES;
         const long long row = row0 + seg * S::V;
         const int n = row >= M ? 0 : (int) (M - row < S::V ? M - row : S::V);
-#pragma unroll
-        for (int p = 0; p < S::PASSES; ++p)
+        if (vecX)
         {
-            const int c = p * S::COLS + tid / S::LANES;
-            *reinterpret_cast<uint4*>(s + at(c) + seg * S::V) = load16(x + (col0 + c) * ldx + row, col0 + c < N ? n : 0, vecX);
+#pragma unroll
+            for (int p = 0; p < S::PASSES; ++p)
+            {
+                const int c = p * S::COLS + tid / S::LANES;
+                const Raw32 r = load32(x + (col0 + c) * ldx + row, col0 + c < N ? n : 0, vecX);
+                uint4* to = reinterpret_cast<uint4*>(s + at(c) + seg * S::V);
+                to[0] = r.a;
+                to[1] = r.b;
+            }
+        }
+        else
+        {
+            // neighbouring threads neighbouring rows, two columns a turn
+            const int r = tid % MX_TILE;
+            const T* px = x + (col0 + tid / MX_TILE) * ldx + row0 + r;
+#pragma unroll 16
+            for (int c = tid / MX_TILE; c < MX_TILE; c += MXT / MX_TILE, px += MXT / MX_TILE * ldx)
+                s[at(c) + r] = row0 + r < M && col0 + c < N ? *px : from_float<T>(0.0f);
         }
     }
     __syncthreads();
@@ -465,50 +591,77 @@ __global__ void __launch_bounds__(MXT, (ACT >= 0 ? 5 : 4)) k_mx_unquantize(const
     const unsigned char* pc = codes + (col0 + c0) * pitch + (FMT == QAGG_MXFP4 ? row / 2 : row);
     const T* pi = in + (col0 + c0) * ldin + row;
     T* po = out + (col0 + c0) * ldout + row;
-    const int cols = n == 0 ? 0 : (int) (N - col0 - c0 < MX_TILE ? N - col0 - c0 : MX_TILE);
+    const int cols = (int) (N - col0 - c0 < MX_TILE ? N - col0 - c0 : MX_TILE); // columns from this thread's first on
+    __shared__ __align__(32) unsigned char rooms[MXT / 32][1024];
+    T* room = reinterpret_cast<T*>(rooms[tid >> 5]);
+    const int lane0 = (tid & 31) / S::LANES;
+    const int rows = (int) (M - row0 < MX_TILE ? M - row0 : MX_TILE);
     if (tid < 32)
         reinterpret_cast<uint4*>(tile)[tid] = __ldcs(reinterpret_cast<const uint4*>(scales + ((long long) blockIdx.y * gridDim.x + blockIdx.x) * 512) + tid);
     __syncthreads();
 #pragma unroll 1
     for (int h = 0; h < MX_TILE; h += S::FLIGHT * S::COLS)
     {
-        unsigned w[S::FLIGHT][2];
-        uint4 raw[ACT >= 0 ? S::FLIGHT : 1];
+        unsigned w[S::FLIGHT][S::V / 4];
+        Raw32 raw[ACT >= 0 ? S::FLIGHT : 1];
 #pragma unroll
         for (int p = 0; p < S::FLIGHT; ++p)
         {
-            const bool have = h + p * S::COLS < cols;
+            const bool have = h + p * S::COLS < cols && n > 0;
             const unsigned char* at = pc + p * S::COLS * pitch;
-            w[p][0] = w[p][1] = 0;
+#pragma unroll
+            for (int q = 0; q < S::V / 4; ++q)
+                w[p][q] = 0;
             if (have)
             {
-                if constexpr (FMT == QAGG_MXFP4 && S::V == 4)
-                    w[p][0] = __ldcs(reinterpret_cast<const unsigned short*>(at));
-                else if constexpr (FMT == QAGG_MXFP4)
+                if constexpr (FMT == QAGG_MXFP4)
                 {
-                    const unsigned q = __ldcs(reinterpret_cast<const unsigned*>(at));
-                    w[p][0] = q & 0xffffu;
-                    w[p][1] = q >> 16;
+                    uint2 q = make_uint2(0, 0);
+                    if constexpr (S::V == 8)
+                        q.x = __ldcs(reinterpret_cast<const unsigned*>(at));
+                    else
+                        q = __ldcs(reinterpret_cast<const uint2*>(at));
+                    w[p][0] = q.x & 0xffffu;
+                    w[p][1] = q.x >> 16;
+                    if constexpr (S::V == 16)
+                    {
+                        w[p][2] = q.y & 0xffffu;
+                        w[p][3] = q.y >> 16;
+                    }
                 }
-                else if constexpr (S::V == 4)
-                    w[p][0] = __ldcs(reinterpret_cast<const unsigned*>(at));
-                else
+                else if constexpr (S::V == 8)
                 {
                     const uint2 q = __ldcs(reinterpret_cast<const uint2*>(at));
                     w[p][0] = q.x;
                     w[p][1] = q.y;
                 }
+                else
+                {
+                    const uint4 q = __ldcs(reinterpret_cast<const uint4*>(at));
+                    w[p][0] = q.x;
+                    w[p][1] = q.y;
+                    w[p][2] = q.z;
+                    w[p][3] = q.w;
+                }
             }
             if constexpr (ACT >= 0)
-                raw[p] = load16(pi + p * S::COLS * ldin, have ? n : 0, vecIn);
+            {
+                const T* at = pi + p * S::COLS * ldin;
+                if (vecIn)
+                    raw[p] = load32(at, have ? n : 0, vecIn);
+                else
+                {
+                    Exchange<T> e;
+                    e.fetch(at - seg * S::V - lane0 * ldin, ldin, rows, cols + lane0 - h - p * S::COLS);
+                    raw[p] = e.take(room);
+                }
+            }
         }
 #pragma unroll
         for (int p = 0; p < S::FLIGHT; ++p)
         {
             const int c = h + p * S::COLS;
-            if (c >= cols)
-                continue;
-            const BlockDecoder<FMT> dec(tile[((c0 + c) & 31) * 16 + ((c0 + c) >> 5) * 4 + b]);
+            const BlockDecoder<FMT> dec(tile[((c0 + c) & 31) * 16 + ((c0 + c) >> 5 & 3) * 4 + b]);
             float v[S::V];
 #pragma unroll
             for (int q = 0; q < S::V / 4; ++q)
@@ -516,12 +669,19 @@ __global__ void __launch_bounds__(MXT, (ACT >= 0 ? 5 : 4)) k_mx_unquantize(const
             if constexpr (ACT >= 0)
             {
                 float g[S::V];
-                unpack16<T>(raw[p], g);
+                unpack32<T>(raw[p], g);
 #pragma unroll
                 for (int i = 0; i < S::V; ++i)
                     v[i] = g[i] * act_slope<ACT>(v[i]);
             }
-            store16(po + p * S::COLS * ldout, v, n, vecOut);
+            T* at = po + p * S::COLS * ldout;
+            if (vecOut)
+            {
+                if (c < cols && n > 0)
+                    store32(at, v, n, vecOut);
+            }
+            else
+                Exchange<T>::put(room, v, at - seg * S::V - lane0 * ldout, ldout, rows, cols + lane0 - c);
         }
         pc += S::FLIGHT * S::COLS * pitch;
         pi += S::FLIGHT * S::COLS * ldin;
@@ -552,7 +712,8 @@ int mx_check_dims(const char* who, long long M, long long N)
 
 static int vec_ok(const void* p, long long ld, int type)
 {
-    return (((uintptr_t) p | (uintptr_t) (ld * mx_type_bytes(type))) & 15) == 0;
+    const uintptr_t low = (uintptr_t) p | (uintptr_t) (ld * mx_type_bytes(type));
+    return (low & 31) == 0 ? VEC32 : (low & 15) == 0 ? VEC16 : 0;
 }
 
 static dim3 tile_grid(long long M, long long N)
