@@ -6,16 +6,18 @@ NCCL: the header and library shipped inside the Python environment (the one PyTo
 present, else the system ones; the library is linked by SONAME (libnccl.so.2), so inside a process that has
 already imported torch the copy torch loaded is reused.
 """
+import concurrent.futures
 import glob
 import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libqagg.so")
-SOURCES = ["qagg_kernels.cu", "qagg_stream.cu", "qagg_unquantize.cu", "qagg_owner.cu", "qagg_capi.cu", "qagg_aggregator.cu", "qagg_dense.cu", "qagg_f64.cu", "qagg_agg_f64.cu", "qagg_update.cu", "qagg_noalloc.cu", "qagg_mx.cu", "qagg_mx_gemm.cu"]
+SOURCES = ["qagg_mx_gemm.cu", "qagg_kernels.cu", "qagg_stream.cu", "qagg_unquantize.cu", "qagg_owner.cu", "qagg_capi.cu", "qagg_aggregator.cu", "qagg_dense.cu", "qagg_f64.cu", "qagg_agg_f64.cu", "qagg_update.cu", "qagg_noalloc.cu", "qagg_mx.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -50,19 +52,27 @@ def build(verbose=False, force=False):
     if not force and not needs_build():
         return OUT
     inc, lib = _nccl_paths()
-    cmd = [nvcc_path(), "-O3", "-std=c++17", "-lineinfo", "--fmad=false", "-shared", "-Xcompiler", "-fPIC,-fvisibility=default"] + ARCH
+    compile_ = [nvcc_path(), "-O3", "-std=c++17", "-lineinfo", "--fmad=false", "-Xcompiler", "-fPIC,-fvisibility=default"] + ARCH
     if verbose:
-        cmd += ["-Xptxas", "-v"]
+        compile_ += ["-Xptxas", "-v"]
     if inc:
-        cmd += ["-I", inc, "-L", lib, "-l:libnccl.so.2", "-Xlinker", "-rpath=" + lib]
-    else:
-        cmd += ["-lnccl"]
-    cmd += ["-o", OUT] + [os.path.join(CSRC, s) for s in SOURCES]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if verbose or res.returncode != 0:
-        sys.stderr.write(" ".join(cmd) + "\n" + res.stdout + res.stderr)
-    if res.returncode != 0:
-        raise RuntimeError("nvcc failed building libqagg.so")
+        compile_ += ["-I", inc]
+    link = [nvcc_path(), "-shared", "-Xcompiler", "-fPIC"] + ARCH
+    link += ["-L", lib, "-l:libnccl.so.2", "-Xlinker", "-rpath=" + lib] if inc else ["-lnccl"]
+
+    def run(cmd):
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if verbose or res.returncode != 0:
+            sys.stderr.write(" ".join(cmd) + "\n" + res.stdout + res.stderr)
+        if res.returncode != 0:
+            raise RuntimeError("nvcc failed building libqagg.so")
+
+    # one compiler per source at a time: the products' file takes as long as all others together
+    with tempfile.TemporaryDirectory() as tmp:
+        objects = [os.path.join(tmp, s.replace(".cu", ".o")) for s in SOURCES]
+        with concurrent.futures.ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+            list(pool.map(run, (compile_ + ["-c", "-o", o, os.path.join(CSRC, s)] for o, s in zip(objects, SOURCES))))
+        run(link + ["-o", OUT] + objects)
     return OUT
 
 

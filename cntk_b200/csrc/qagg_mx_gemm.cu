@@ -77,7 +77,7 @@ __device__ __forceinline__ void split_range(int steps, int rank, int splits, int
     count = (int) ((long long) steps * (rank + 1) / splits) - first;
 }
 
-// After a wait ran out: the copies this thread started have landed (or a bounded wait for them ran out too) before the CTA goes.
+// The copies this thread started have landed, after a wait ran out too (or a bounded wait for them ran out as well), before the CTA goes.
 __device__ __forceinline__ void drain_copies(GemmBars* bars, long long issued, int stages)
 {
     const unsigned long long began = clock_ns();
@@ -375,8 +375,6 @@ struct TimesArgs
 constexpr int TT = 384;  // copy, product, allocating and spare warp; eight result warps
 constexpr int TIMES_NARROW = 32;
 constexpr int TK = 256;  // contraction values per stage: 128 bytes of codes
-
-
 constexpr int TIMES_PAIR = 256; // width of a tile that two CTAs make
 // codes of 128 rows of W and `rows` of X, scales of W's and of bn of X's
 __host__ __device__ inline int times_stage_bytes(int bn, int rows)
@@ -473,7 +471,6 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
                         tc_wait(&bars.empty[ring.s], ring.par ^ 1, &bars.broken, &g_mxStatus);
                     if (*reinterpret_cast<volatile unsigned*>(&bars.broken))
                     {
-                        drain_copies(&bars, issued, S);
                         tile = a.tiles;
                         break;
                     }
@@ -481,6 +478,7 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
                     ring.next(S);
                 }
             }
+            drain_copies(&bars, issued, S);
         }
     }
     else if (warp == 1 && (!PAIR || rank == 0))
@@ -1063,7 +1061,6 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
                         tc_wait(&bars.empty[ring.s], ring.par ^ 1, &bars.broken, &g_mxStatus);
                     if (*reinterpret_cast<volatile unsigned*>(&bars.broken))
                     {
-                        drain_copies(&bars, issued, S);
                         tile = a.tiles;
                         break;
                     }
@@ -1071,6 +1068,7 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
                     ring.next(S);
                 }
             }
+            drain_copies(&bars, issued, S);
         }
         else if (warp == 1 && (!PAIR || rank == 0) && elect_one())
         {
