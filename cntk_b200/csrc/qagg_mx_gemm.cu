@@ -825,7 +825,8 @@ constexpr int GRAD_SCALE_BYTES = 512, GRAD_SCALE_ROOM = 1024; // stages stay mul
 // contraction values k..k+3; pair 0 is (k, k + 1), pair 1 (k + 2, k + 3).
 // int8: 0x43 over a code byte is the bf16 number 128 + (its low seven bits) with bit 7 moved aside; q = low - (bit 7), so
 // q = (128 + low) - (128 or 256), and 256 is 0x4380.  fp4: the element's exponent and mantissa bits, set where bf16 has them, give
-// its value times 2^-126, subnormal included.  All products are exact.
+// its value times 2^-126, subnormal included; one multiplication puts two copies of a nibble where sign and the rest belong.  The
+// multiplier has the 2^126 in it (X <= 1: largest magnitudes below 16) or the step takes two.  All products are exact.
 __device__ __forceinline__ unsigned bf16x2_mul(unsigned a, unsigned b)
 {
     const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
@@ -841,16 +842,19 @@ __device__ __forceinline__ unsigned expand_int8(unsigned v, int pair, unsigned s
     const unsigned x = __byte_perm(v, 0x43434343u, pair ? 0x4342 : 0x4140);
     return bf16x2_mul(bf16x2_sub(x & 0xff7fff7fu, x & 0xff80ff80u), scale);
 }
-__device__ __forceinline__ unsigned expand_fp4(unsigned v, int pair, bool odd, unsigned scale)
+__device__ __forceinline__ unsigned expand_fp4(unsigned v, int pair, bool odd, bool large, unsigned scale)
 {
     const unsigned x = __byte_perm(v, 0, pair ? 0x4342 : 0x4140);
-    const unsigned t = odd ? ((x << 2) & 0x01c001c0u) | ((x << 8) & 0x80008000u) : ((x << 6) & 0x01c001c0u) | ((x << 12) & 0x80008000u);
-    return bf16x2_mul(bf16x2_mul(t, 0x7e807e80u), scale); // 2^126
+    const unsigned t = (odd ? (x & 0x00f000f0u) * 0x104u : (x & 0x000f000fu) * 0x1040u) & 0x81c081c0u;
+    return large ? bf16x2_mul(bf16x2_mul(t, 0x7e807e80u), scale) : bf16x2_mul(t, scale); // 0x7e80: 2^126
 }
-// multiplier of a block as bf16 bits: 2^X (fp4), 2^X / 64 (int8; subnormal below byte 7)
+// multiplier of a block as bf16 bits: 2^X / 64 (int8; subnormal below byte 7), 2^X or 2^(X + 126) (fp4)
+constexpr unsigned FP4_LARGE = 128; // scale bytes above this have no 2^(X + 126)
 template <int FMT>
-__device__ __forceinline__ unsigned scale_bf16(unsigned byte)
+__device__ __forceinline__ unsigned scale_bf16(unsigned byte, bool large)
 {
+    if (FMT == QAGG_MXFP4 && !large)
+        return (byte + 126u) << 7;
     if (byte == 255u)
         return 0x7fffu;
     if (FMT == QAGG_MXINT8)
@@ -1179,8 +1183,10 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
                     ldmatrix_trans_b8(rowAt[h] + off + 32 * ROW, reinterpret_cast<unsigned(&)[4]>(c[h][4]));
                 }
                 const unsigned char* sb = scaleAt + off + ((first + i) & 1) * 8;
-                mult[lane] = (unsigned short) scale_bf16<FMT>(sb[0]);
-                mult[lane + 32] = (unsigned short) scale_bf16<FMT>(sb[4]);
+                const unsigned b0 = sb[0], b1 = sb[4];
+                const bool large = FMT == QAGG_MXFP4 && __any_sync(0xffffffffu, b0 > FP4_LARGE || b1 > FP4_LARGE);
+                mult[lane] = (unsigned short) scale_bf16<FMT>(b0, large);
+                mult[lane + 32] = (unsigned short) scale_bf16<FMT>(b1, large);
                 __syncwarp();
                 uint2 sc[4]; // multipliers of contraction values 16 g + 4 (lane % 4) .. + 3
 #pragma unroll
@@ -1193,21 +1199,28 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
                 }
                 tc_fence_after();
                 const unsigned to = tmA + ((unsigned) (quad * 32) << 16) + slot * 32;
+                const auto expand = [&](auto large_) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                {
-                    unsigned r[16];
+                    for (int h = 0; h < 2; ++h)
+                    {
+                        unsigned r[16];
 #pragma unroll
-                    for (int g = 0; g < 4; ++g)
+                        for (int g = 0; g < 4; ++g)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) // rows l / 4, l / 4 + 8 of the half
-                        {
-                            const unsigned v = FMT == QAGG_MXINT8 ? c[h % HALVES][2 * g + e] : c[0][2 * g + h];
-                            r[4 * g + 2 * e] = FMT == QAGG_MXINT8 ? expand_int8(v, 0, sc[g].x) : expand_fp4(v, 0, e, sc[g].x);
-                            r[4 * g + 2 * e + 1] = FMT == QAGG_MXINT8 ? expand_int8(v, 1, sc[g].y) : expand_fp4(v, 1, e, sc[g].y);
-                        }
-                    tmem_store_16x256b(to + ((unsigned) (h * 16) << 16), r);
-                }
+                            for (int e = 0; e < 2; ++e) // rows l / 4, l / 4 + 8 of the half
+                            {
+                                const unsigned v = FMT == QAGG_MXINT8 ? c[h % HALVES][2 * g + e] : c[0][2 * g + h];
+                                constexpr bool LARGE = decltype(large_)::value;
+                                r[4 * g + 2 * e] = FMT == QAGG_MXINT8 ? expand_int8(v, 0, sc[g].x) : expand_fp4(v, 0, e, LARGE, sc[g].x);
+                                r[4 * g + 2 * e + 1] = FMT == QAGG_MXINT8 ? expand_int8(v, 1, sc[g].y) : expand_fp4(v, 1, e, LARGE, sc[g].y);
+                            }
+                        tmem_store_16x256b(to + ((unsigned) (h * 16) << 16), r);
+                    }
+                };
+                if (FMT == QAGG_MXFP4 && large)
+                    expand(std::true_type());
+                else
+                    expand(std::false_type());
                 tmem_store_wait();
                 tc_fence_before();
                 __syncwarp();
