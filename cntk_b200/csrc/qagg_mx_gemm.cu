@@ -785,6 +785,7 @@ struct GradArgs
     int vec;            // dy can be read 16 bytes a time
     int wide, wide4;    // out: rows can be written 16 bytes a time, columns in pairs of rows; four neighbours at once
     int add;
+    int pair;
 };
 
 constexpr int GK = 64; // contraction values per stage
@@ -794,7 +795,7 @@ constexpr int GK = 64; // contraction values per stage
 // each as the SM has for all of them, and redistribute them.
 // PAIR: two CTAs make a 256 x 256 tile together, each with 128 rows of the packed operand and half of dy's columns, so that each brings
 // 24 KB (int8; fp4 20) for 512 cycles of products where a CTA by itself brings 32 (28) for 384: copies from L2, at some 46
-// bytes a cycle, are what bounds these kernels.
+// bytes a cycle, are what bounds these kernels.  With loaders the tile is 256 x 128, and each CTA splits 64 of the columns.
 // Tensor memory: two accumulators of 192 columns and four expanded steps of 32, or, tiles being 128 wide with loaders, two of 128
 // and eight.  A 192-wide tile reads 6 % more per product than one of 256, which would leave room for one accumulator.  A pair has one
 // of 256 columns, and eight expanded steps.
@@ -802,15 +803,16 @@ constexpr int GRAD_WIDEST = 192, GRAD_WIDEST_DENSE = 128, GRAD_PAIR = 256;
 template <bool DENSE, bool PAIR>
 struct GradGroups
 {
-    static constexpr int expand = DENSE ? 1 : PAIR ? 2 : 3, result = DENSE ? 1 : 2, load = DENSE ? 4 : 0;
+    static constexpr int expand = DENSE ? (PAIR ? 2 : 1) : PAIR ? 2 : 3, result = DENSE ? 1 : 2, load = DENSE ? 4 : 0;
     static constexpr int firstExpand = 4, firstResult = firstExpand + 4 * expand, firstLoad = firstResult + 4 * result;
     static constexpr int threads = 128 * (1 + expand + result + load);
-    static constexpr int regsLaunch = DENSE ? 72 : PAIR ? 96 : 80; // 65536 / threads, a multiple of 8
-    static constexpr int regsMisc = DENSE ? 40 : PAIR ? 48 : 56, regsExpand = PAIR ? 64 : 56, regsResult = DENSE || PAIR ? 152 : 128, regsLoad = 64;
+    static constexpr int regsLaunch = DENSE ? (PAIR ? 64 : 72) : PAIR ? 96 : 80; // 65536 / threads, a multiple of 8
+    static constexpr int regsMisc = DENSE ? 40 : PAIR ? 48 : 56, regsExpand = DENSE && PAIR ? 48 : PAIR ? 64 : 56, regsResult = DENSE || PAIR ? 152 : 128,
+                         regsLoad = PAIR ? 56 : 64;
     static_assert(regsLaunch * threads <= 65536 && 128 * (regsMisc + regsExpand * expand + regsResult * result + regsLoad * load) <= regsLaunch * threads, "registers");
     static constexpr int widest = DENSE ? GRAD_WIDEST_DENSE : PAIR ? GRAD_PAIR : GRAD_WIDEST;
-    static constexpr int accumulators = PAIR ? 1 : 2;
-    static constexpr unsigned side = accumulators * widest;      // first column behind the accumulators
+    static constexpr int accumulators = PAIR && !DENSE ? 1 : 2;
+    static constexpr unsigned side = accumulators * widest;     // first column behind the accumulators
     static constexpr int slots = (int) (TMEM_COLS - side) / 32; // expanded steps in tensor memory
 };
 
@@ -919,9 +921,8 @@ template <bool WEIGHT, int FMT, int DENSE, bool PAIR, class TD, class TO>
 __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_mx_grad(const __grid_constant__ CUtensorMap mapCodes, const __grid_constant__ CUtensorMap mapDy, const GradArgs a)
 {
     using G = GradGroups<(DENSE > 0), PAIR>;
-    static_assert(!(PAIR && DENSE), "pairs bring dy through the copy engine");
     constexpr int NP = DENSE ? DENSE : 1;
-    constexpr int CHAIN_STEPS = (sizeof(TO) != 4 ? CHAIN_16BIT : PAIR ? CHAIN_SINGLE : CHAIN) / 4 / NP;
+    constexpr int CHAIN_STEPS = (sizeof(TO) != 4 ? CHAIN_16BIT : G::accumulators == 1 ? CHAIN_SINGLE : CHAIN) / 4 / NP;
     constexpr int WIDEST = G::widest, SLOTS = G::slots, BUFS = G::accumulators;
     extern __shared__ unsigned char dyn[];
     __shared__ GemmBars bars;
@@ -974,7 +975,7 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
     int early = 0; // steps of the first tile whose copies start before the CTA has met
     if (warp == 0)
     {
-        init_barriers(&bars, S, PAIR ? 8 : 4, 4 * G::load, PAIR ? 2 * resultWarps : resultWarps);
+        init_barriers(&bars, S, PAIR ? 8 : 4, 4 * G::load * (PAIR ? 2 : 1), PAIR ? 2 * resultWarps : resultWarps);
         if (elect_one())
         {
             const Source src = source_of(firstTile);
@@ -985,12 +986,13 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
         __syncwarp();
     }
     // Loaders of the dense operand: rows of 64 contiguous values (128 bytes a plane), in units of eight values.  A thread has two units a
-    // step, the second 64 columns (rows of 64 tokens) further: 8192 bytes in the stage, a constant in memory.
-    constexpr int THREADS = DENSE ? 128 * G::load : 512;
+    // step (one of a pair's, which has half of the columns), the second 64 columns (rows of 64 tokens) further: 8192 bytes in the
+    // stage, a constant in memory.
+    constexpr int THREADS = DENSE ? 128 * G::load : 512, UNITS = PAIR ? 1 : 2;
     static_assert(THREADS * 2 == GRAD_WIDEST_DENSE * 8, "two units a thread");
     struct Units
     {
-        Raw8<TD> raw[2];
+        Raw8<TD> raw[UNITS];
     };
     const int unit = threadIdx.x - G::firstLoad * 32; // 8 row + piece of the row
     const long long unitStride = WEIGHT ? 64 : 64 * a.ldDy, stepStride = WEIGHT ? GK * a.ldDy : GK;
@@ -1004,7 +1006,7 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
         if (nextStep == 0)
         {
             const int c = (unit & 7) * 8, r = unit >> 3;
-            const long long n0 = tile_n0(nextTile), k0 = (long long) first * GK;
+            const long long n0 = tile_n0(nextTile) + (PAIR ? rank * share : 0), k0 = (long long) first * GK;
             const long long line = (WEIGHT ? k0 : n0) + r, col = (WEIGHT ? n0 : k0) + c; // token, output
             from = (const TD*) a.dy + line * a.ldDy + col;
             left = (int) (a.C - k0) - (WEIGHT ? r : c);
@@ -1012,17 +1014,18 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
             {
                 const long long cols = a.N - col;
                 have0 = (int) (cols < 0 ? 0 : cols < 8 ? cols : 8);
-                have1 = bn <= 64 || cols <= 64 ? 0 : (int) (cols < 72 ? cols - 64 : 8);
+                have1 = share <= 64 || cols <= 64 ? 0 : (int) (cols < 72 ? cols - 64 : 8);
             }
             else
             {
                 have0 = line < a.N ? 8 : 0;
-                have1 = bn > 64 && line + 64 < a.N ? 8 : 0;
+                have1 = share > 64 && line + 64 < a.N ? 8 : 0;
             }
         }
         const int most = WEIGHT ? (left > 0 ? 8 : 0) : left < 0 ? 0 : left < 8 ? left : 8;
         v.raw[0] = load8(from, min(have0, most), a.vec);
-        v.raw[1] = load8(from + unitStride, min(have1, most), a.vec);
+        if constexpr (UNITS == 2)
+            v.raw[UNITS - 1] = load8(from + unitStride, min(have1, most), a.vec);
         from += stepStride;
         left -= GK;
         if (++nextStep == count)
@@ -1103,9 +1106,9 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
 #pragma unroll
                         for (int j = 0; j < GK / 16; ++j)
                             if constexpr (PAIR)
-                                mma_bf16_ts_pair(acc, ta + j * 8, d + j * KSTEP, idesc, inChain > 0 || j > 0);
+                                mma_bf16_ts_pair(acc, ta + j * 8, d + p * (share * 128 >> 4) + j * KSTEP, idesc, inChain > 0 || p + j > 0);
                             else
-                                mma_bf16_ts(acc, ta + j * 8, d + p * (bn * 128 >> 4) + j * KSTEP, idesc, inChain > 0 || p + j > 0);
+                                mma_bf16_ts(acc, ta + j * 8, d + p * (share * 128 >> 4) + j * KSTEP, idesc, inChain > 0 || p + j > 0);
                     if constexpr (PAIR)
                         tc_commit_pair(&bars.empty[ring.s]);
                     else
@@ -1290,7 +1293,7 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
             ++done;
             unsigned char* at = mine + ring.s * stageBytes;
 #pragma unroll
-            for (int q = 0; q < 2; ++q)
+            for (int q = 0; q < UNITS; ++q)
             {
                 unsigned w[NP][4];
                 if (NP == 1)
@@ -1299,15 +1302,20 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
                     split8<TD, NP, true>(v.raw[q], w);
                 else
                     split8<TD, NP, false>(v.raw[q], w);
-                if (q == 0 || bn > 64)
+                if (q == 0 || share > 64)
 #pragma unroll
                     for (int p = 0; p < NP; ++p)
-                        *reinterpret_cast<uint4*>(at + q * 8192 + p * bn * 128) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+                        *reinterpret_cast<uint4*>(at + q * 8192 + p * share * 128) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
             }
             fence_async_shared();
             __syncwarp();
             if (lane == 0)
-                mbar_arrive(&bars.dense[ring.s]);
+            {
+                if constexpr (PAIR)
+                    mbar_arrive_remote(&bars.dense[ring.s], 0);
+                else
+                    mbar_arrive(&bars.dense[ring.s]);
+            }
             ring.next(S);
         };
         const long long mySteps = firstTile < a.tiles ? (long long) ((a.tiles - 1 - firstTile) / tileStep + 1) * count : 0;
@@ -1424,13 +1432,14 @@ template <bool WEIGHT, int FMT, int DENSE, class TD, class TO>
 static cudaError_t launch_grad(cudaStream_t st, const CUtensorMap& mc, const CUtensorMap& md, GradArgs a, int sms)
 {
     constexpr int NP = DENSE ? DENSE : 1;
-    if constexpr (DENSE == 0)
-        if (a.bn == GRAD_PAIR)
+    if constexpr (WEIGHT || DENSE == 0 || std::is_same_v<TD, TO> || std::is_same_v<TO, float>)
+        if (a.pair)
         {
-            const int stageBytes = GRAD_PAIR / 2 * 128 + grad_codes_bytes(FMT) + GRAD_SCALE_ROOM;
+            const int stageBytes = a.bn / 2 * 128 * NP + grad_codes_bytes(FMT) + GRAD_SCALE_ROOM;
             a.stages = stages_for(stageBytes, MAX_STAGES);
             const int smem = smem_for(stageBytes, a.stages, 0);
-            return launch_cluster<k_mx_grad<WEIGHT, FMT, 0, true, TD, TO>>(dim3((unsigned) (2 * std::min(a.tiles, sms / 2))), GradGroups<false, true>::threads, smem, dim3(2, 1, 1), st, mc, md, a);
+            return launch_cluster<k_mx_grad<WEIGHT, FMT, DENSE, true, TD, TO>>(dim3((unsigned) (2 * std::min(a.tiles, sms / 2))), GradGroups<(DENSE > 0), true>::threads, smem,
+                                                                              dim3(2, 1, 1), st, mc, md, a);
         }
     const int stageBytes = a.bn * 128 * NP + grad_codes_bytes(FMT) + GRAD_SCALE_ROOM;
     a.stages = stages_for(stageBytes, MAX_STAGES);
@@ -1449,13 +1458,14 @@ static cudaError_t launch_grad_dense(cudaStream_t st, const CUtensorMap& mc, con
     return launch_grad<WEIGHT, FMT, 3, float, TO>(st, mc, md, a, sms);
 }
 
-// Two CTAs on a 256 x 256 tile, or one on 128 x bn: cycles as in choose_shape, with what a pair waits for its one accumulator.
-static bool pair_pays(long long I, long long N, const GradArgs& a, int sms, int format)
+// Two CTAs on a 256 x 256 (with loaders 256 x 128) tile, or one on 128 x bn: cycles as in choose_shape, with what a pair waits for its
+// one accumulator.  Loaders and splitting warps take a CTA by itself 2000 cycles a step of 128 columns, each of a pair 1200.
+static bool pair_pays(long long I, long long N, const GradArgs& a, int sms, int format, bool tma)
 {
-    const int codes = grad_codes_bytes(format);
-    const double one = std::max(2.0 * a.bn, (codes + a.bn * 128.0) / 46.0) * ((a.tiles + sms - 1) / sms);
-    const long long pairs = (I + 255) / 256 * ((N + 255) / 256);
-    const double two = std::max(512.0, (codes + 16384.0) / 46.0) * 1.25 * ((pairs + sms / 2 - 1) / (sms / 2));
+    const int codes = grad_codes_bytes(format), width = tma ? GRAD_PAIR : GRAD_WIDEST_DENSE;
+    const double one = (tma ? std::max(2.0 * a.bn, (codes + a.bn * 128.0) / 46.0) : 2000.0) * ((a.tiles + sms - 1) / sms);
+    const long long pairs = (I + 255) / 256 * ((N + width - 1) / width);
+    const double two = (tma ? std::max(512.0, (codes + 16384.0) / 46.0) * 1.25 : 1200.0) * ((pairs + sms / 2 - 1) / (sms / 2));
     return two < one;
 }
 
@@ -1504,11 +1514,13 @@ static int grad_common(const char* who, bool weight, void* stream, const void* d
     a.splits = sh.splits;
     a.tilesM = (int) ((I + 127) / 128);
     a.tiles = a.tilesM * (int) ((N + a.bn - 1) / a.bn);
-    if (tma && a.splits == 1 && pair_pays(I, N, a, cfg.numSMs, format))
+    // with loaders a pair's kernel exists for outputs of dy's type and fp32 (and is not worth one more for the others)
+    if (a.splits == 1 && (tma || weight || outType == dyType || outType == QAGG_F32) && pair_pays(I, N, a, cfg.numSMs, format, tma))
     {
-        a.bn = GRAD_PAIR;
+        a.pair = 1;
+        a.bn = tma ? GRAD_PAIR : GRAD_WIDEST_DENSE;
         a.tilesM = (int) ((I + 255) / 256);
-        a.tiles = a.tilesM * (int) ((N + GRAD_PAIR - 1) / GRAD_PAIR);
+        a.tiles = a.tilesM * (int) ((N + a.bn - 1) / a.bn);
     }
     a.wide = weight ? ((((uintptr_t) out | (uintptr_t) (ldOut * 4)) & 15) == 0) : ((uintptr_t) out & 3) == 0 && (ldOut & 1) == 0;
     a.wide4 = (((uintptr_t) out | (uintptr_t) (ldOut * mx_type_bytes(outType))) & (4 * mx_type_bytes(outType) - 1)) == 0;
@@ -1517,7 +1529,7 @@ static int grad_common(const char* who, bool weight, void* stream, const void* d
     std::memset(&md, 0, sizeof(md));
     if (C > 0 && !codes_map(&mc, codes, I, C, format, format == QAGG_MXFP4 ? 64 : 128, GK))
         return fail(QAGG_ECUDA, std::string(who) + ": tensor map of the codes could not be made");
-    if (C > 0 && tma && !encode_map_tiled(&md, 2, dy, O, T, ldDy * 2, 64, weight ? GK : a.bn == GRAD_PAIR ? GRAD_PAIR / 2 : a.bn, 128))
+    if (C > 0 && tma && !encode_map_tiled(&md, 2, dy, O, T, ldDy * 2, 64, weight ? GK : a.pair ? a.bn / 2 : a.bn, 128))
         return fail(QAGG_ECUDA, std::string(who) + ": tensor map of dy could not be made");
     const cudaStream_t st = (cudaStream_t) stream;
     cudaError_t e;

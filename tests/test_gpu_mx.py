@@ -272,9 +272,10 @@ def test_input_grad(lib, O, I, T, pad, offset, t, fmt):
 
 
 @pytest.mark.parametrize("t", ["bf16", "f16", "f32"])
-@pytest.mark.parametrize("O,I,T", [(2048, 1100, 2100), (2049, 1100, 2100)])
+@pytest.mark.parametrize("O,I,T", [(2048, 1100, 2100), (2049, 1100, 2100), (2301, 1100, 900), (2304, 1300, 900)])
 def test_more_tiles_than_sms(lib, O, I, T, t):
-    """Several tiles per CTA, with and without 16-byte columns of dy."""
+    """Several tiles per CTA, by single CTAs and by pairs, the last pair with and without rows for its second CTA; with and without
+    16-byte columns of dy."""
     rng = np.random.default_rng(O)
     _, d, dy = dense(rng, T, O, t, 0, 0, 1e-2)
     planes = {"bf16": 1, "f16": 2, "f32": 3}[t]
