@@ -144,6 +144,20 @@ def test_quantize_borders(lib, fmt, transpose):
     assert np.array_equal(got, values, equal_nan=True)
 
 
+@pytest.mark.parametrize("fmt", [mx_util.FP4, mx_util.INT8])
+@pytest.mark.parametrize("m,n,pad,offset", [(96, 40, 0, 0), (77, 33, 2, 1)])
+def test_values_in_half_precision(lib, m, n, pad, offset, fmt):
+    """fp16 cannot hold every value: each is rounded to nearest, too large ones to infinity."""
+    rng = np.random.default_rng(15)
+    x = rng.standard_normal((n, m)) * np.exp2(rng.integers(-30, 20, (n, 1)))
+    (codes, scales), v = to_dev(*mx_util.pack(x, fmt)), mx_util.values(x, fmt)
+    flat, out = room(n, m, "f16", pad, offset)
+    lib.mx_unquantize(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), lib.F16, m + pad, m, n, fmt, stream())
+    with np.errstate(over="ignore"):
+        assert np.array_equal(out.cpu().numpy(), v.astype(np.float16))
+    untouched(flat, out, pad, offset)
+
+
 def test_offsets_beyond_32_bits(lib):
     """The last columns of a matrix of more than 2^32 values, with a gap between the columns."""
     m, n, ld = 64, 3, (1 << 31) + 64
@@ -181,6 +195,29 @@ def test_times(lib, O, T, K, pad, t):
         lib.mx_check(stream())
         check(y, want, mags + (np.abs(bias) if b else 0), K / 16, t, f"times {O}x{T}x{K}")
         untouched(flat, y, pad, 0)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("O,T,K,pad,offset", [(256, 130, 300, 0, 1), (256, 40, 2048, 2, 1), (256, 40, 2048, 4, 2), (2304, 2500, 300, 2, 3)])
+def test_results_at_any_alignment(lib, O, T, K, pad, offset, t):
+    """Bases and distances between columns that rule out the wider stores, in whole and in split products."""
+    rng = np.random.default_rng(21)
+    (wc, ws), w = packed(rng, O, K, mx_util.FP4, 0.05)
+    (xc, xs), x = packed(rng, T, K, mx_util.FP4)
+    flat, y = room(T, O, t, pad, offset)
+    lib.mx_times(wc.data_ptr(), ws.data_ptr(), xc.data_ptr(), xs.data_ptr(), 0, y.data_ptr(), code(lib, t), O + pad, O, T, K, stream())
+    check(y, x @ w.T, np.abs(x) @ np.abs(w).T, K / 16, t, "times")
+    untouched(flat, y, pad, offset)
+    # the gradients of the same layer
+    _, d, dy = dense(rng, T, O, "bf16", 0, 0, 1e-2)
+    flat, dw = room(K, O, "f32", 0, offset)
+    lib.mx_weight_grad(d.data_ptr(), lib.BF16, O, xc.data_ptr(), xs.data_ptr(), 4, dw.data_ptr(), O, K, T, False, stream())
+    check(dw, x.T @ dy, np.abs(x).T @ np.abs(dy), T / 16, "f32", "weight gradient")
+    untouched(flat, dw, 0, offset)
+    flat, dx = room(T, K, t, pad, offset)
+    lib.mx_input_grad(d.data_ptr(), lib.BF16, O, wc.data_ptr(), ws.data_ptr(), 4, dx.data_ptr(), code(lib, t), K + pad, O, K, T, stream())
+    check(dx, dy @ w, np.abs(dy) @ np.abs(w), O / 16, t, "input gradient")
+    untouched(flat, dx, pad, offset)
 
 
 def test_times_without_inputs_is_the_bias(lib):
@@ -403,6 +440,29 @@ def test_activation(lib, m, n, pad, offset, t, act):
         tol = 12 * 2.0 ** -24 * size + eps / 2 * np.abs(ref) + (2.0 ** -25 if t == "f16" else 0)
         err = np.abs(got.double().cpu().numpy() - ref)
         assert (err <= tol).all(), f"worst {np.max(err / tol)}"
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("pads", [(0, 3), (3, 0), (16, 8), (8, 5)])
+def test_activation_with_columns_of_different_distances(lib, pads, t):
+    """x and y (dy and dx) aligned and not, in every combination; values of the aligned call."""
+    m, n = 160, 70
+    rng = np.random.default_rng(12)
+    _, d, x = dense(rng, n, m, t, pads[0], 0, 2.0)
+    same = [torch.zeros(lib.mx_code_bytes(m, n, 8), dtype=torch.uint8, device=DEV), torch.zeros(lib.mx_scale_bytes(m, n), dtype=torch.uint8, device=DEV)]
+    flat, y = room(n, m, t, pads[1])
+    lib.mx_act_forward(d.data_ptr(), code(lib, t), m + pads[0], lib.ACT_SILU, y.data_ptr(), m + pads[1], same[0].data_ptr(), same[1].data_ptr(), m, n, stream())
+    flat2, dx = room(n, m, t, pads[1])
+    lib.mx_act_backward(d.data_ptr(), code(lib, t), m + pads[0], same[0].data_ptr(), same[1].data_ptr(), lib.ACT_SILU, dx.data_ptr(), m + pads[1], m, n, stream())
+    untouched(flat, y, pads[1], 0)
+    untouched(flat2, dx, pads[1], 0)
+    near = d.contiguous()
+    codes, scales, y0, dx0 = torch.zeros_like(same[0]), torch.zeros_like(same[1]), torch.zeros_like(near), torch.zeros_like(near)
+    lib.mx_act_forward(near.data_ptr(), code(lib, t), m, lib.ACT_SILU, y0.data_ptr(), m, codes.data_ptr(), scales.data_ptr(), m, n, stream())
+    lib.mx_act_backward(near.data_ptr(), code(lib, t), m, codes.data_ptr(), scales.data_ptr(), lib.ACT_SILU, dx0.data_ptr(), m, m, n, stream())
+    want = mx_util.pack(x, 8)
+    assert np.array_equal(codes.cpu().numpy(), want[0]) and np.array_equal(scales.cpu().numpy(), want[1])
+    assert torch.equal(codes, same[0]) and torch.equal(scales, same[1]) and torch.equal(y, y0) and torch.equal(dx, dx0)
 
 
 @pytest.mark.parametrize("act", range(5))
