@@ -19,6 +19,7 @@
 // Where there are fewer tiles than SMs the contraction is split over the CTAs of a cluster, whose partial sums are added through
 // distributed shared memory in rank order: no workspace, no atomics, the same bits on every run.
 #include "qagg_mx.cuh"
+#include "qagg_mx_groups.h"
 #include "qagg_tcgen05.cuh"
 
 #include <algorithm>
@@ -32,7 +33,6 @@ namespace qagg {
 // set by a bounded wait that ran out; read and cleared by qagg_mx_check
 __device__ unsigned g_mxStatus;
 
-constexpr unsigned TMEM_COLS = 512; // accumulators first; behind them block scales or expanded operands
 constexpr int MAX_STAGES = 8;
 constexpr int GEMM_SMEM_MAX = 224 * 1024; // dynamic; barriers and scales take a little more
 // Nearly all of an SM's shared memory, always: a second CTA on the SM, of these kernels or of any other that uses tensor memory, would
@@ -790,32 +790,6 @@ struct GradArgs
 
 constexpr int GK = 64; // contraction values per stage
 
-// Threads, in groups of four warps: copy / product / allocating / spare; expanding; result; with a dense operand that the copy engine
-// cannot take, one group less of the second and third kind and four of loaders.  The threads are launched with as many registers
-// each as the SM has for all of them, and redistribute them.
-// PAIR: two CTAs make a 256 x 256 tile together, each with 128 rows of the packed operand and half of dy's columns, so that each brings
-// 24 KB (int8; fp4 20) for 512 cycles of products where a CTA by itself brings 32 (28) for 384: copies from L2, at some 46
-// bytes a cycle, are what bounds these kernels.  With loaders the tile is 256 x 128, and each CTA splits 64 of the columns.
-// Tensor memory: two accumulators of 192 columns and four expanded steps of 32, or, tiles being 128 wide with loaders, two of 128
-// and eight.  A 192-wide tile reads 6 % more per product than one of 256, which would leave room for one accumulator.  A pair has one
-// of 256 columns, and eight expanded steps.
-constexpr int GRAD_WIDEST = 192, GRAD_WIDEST_DENSE = 128, GRAD_PAIR = 256;
-template <bool DENSE, bool PAIR>
-struct GradGroups
-{
-    static constexpr int expand = DENSE ? (PAIR ? 2 : 1) : PAIR ? 2 : 3, result = DENSE ? 1 : 2, load = DENSE ? 4 : 0;
-    static constexpr int firstExpand = 4, firstResult = firstExpand + 4 * expand, firstLoad = firstResult + 4 * result;
-    static constexpr int threads = 128 * (1 + expand + result + load);
-    static constexpr int regsLaunch = DENSE ? (PAIR ? 64 : 72) : PAIR ? 96 : 80; // 65536 / threads, a multiple of 8
-    static constexpr int regsMisc = DENSE ? 40 : PAIR ? 48 : 56, regsExpand = DENSE && PAIR ? 48 : PAIR ? 64 : 56, regsResult = DENSE || PAIR ? 152 : 128,
-                         regsLoad = PAIR ? 56 : 64;
-    static_assert(regsLaunch * threads <= 65536 && 128 * (regsMisc + regsExpand * expand + regsResult * result + regsLoad * load) <= regsLaunch * threads, "registers");
-    static constexpr int widest = DENSE ? GRAD_WIDEST_DENSE : PAIR ? GRAD_PAIR : GRAD_WIDEST;
-    static constexpr int accumulators = PAIR && !DENSE ? 1 : 2;
-    static constexpr unsigned side = accumulators * widest;     // first column behind the accumulators
-    static constexpr int slots = (int) (TMEM_COLS - side) / 32; // expanded steps in tensor memory
-};
-
 // packed part of a stage: 64 contraction values x 128 rows of codes, and the scale tile they lie in (128 values x 128 rows)
 __host__ __device__ inline int grad_codes_bytes(int format)
 {
@@ -939,7 +913,6 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
     if (!PAIR)
         split_range(steps, rank, a.splits, first, count);
     const int firstTile = PAIR ? blockIdx.x >> 1 : blockIdx.x, tileStep = PAIR ? gridDim.x >> 1 : gridDim.x;
-    constexpr int resultWarps = 4 * G::result;
     auto tile_m0 = [&](int tile) { return (long long) (tile % a.tilesM) * (PAIR ? 256 : 128) + (PAIR ? rank * 128 : 0); };
     auto tile_n0 = [&](int tile) { return (long long) (tile / a.tilesM) * bn; };
 
@@ -975,7 +948,7 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
     int early = 0; // steps of the first tile whose copies start before the CTA has met
     if (warp == 0)
     {
-        init_barriers(&bars, S, PAIR ? 8 : 4, 4 * G::load * (PAIR ? 2 : 1), PAIR ? 2 * resultWarps : resultWarps);
+        init_barriers(&bars, S, G::convArrivals, G::denseArrivals, G::takenArrivals);
         if (elect_one())
         {
             const Source src = source_of(firstTile);

@@ -129,3 +129,15 @@ def test_no_cpu_fallback(lib):
         with pytest.raises(lib.QaggError) as e:
             call()
         assert "qagg error -2" in str(e.value)
+
+
+def test_roles_of_the_gradient_products(tmp_path):
+    """Barrier counts, registers and tensor memory of the four ways to divide a CTA, compiled for the host."""
+    import os
+    import subprocess
+    exe = str(tmp_path / "mx_groups_check")
+    src = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "mx_groups_check.cpp")
+    res = subprocess.run(["g++", "-std=c++17", "-O0", src, "-o", exe], capture_output=True, text=True)
+    assert res.returncode == 0, res.stderr
+    run = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert run.returncode == 0 and "groups ok" in run.stdout, (run.returncode, run.stdout)
