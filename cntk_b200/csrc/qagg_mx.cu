@@ -326,7 +326,7 @@ __device__ __forceinline__ float act_value(float x)
     {
         float e;
         const float tail = normal_tail(x, e);
-        return __fmaf_rn(-fabsf(x), tail, fmaxf(x, 0.0f)); // x - x tail or x tail (NaN: tail is)
+        return x * (x < 0.0f ? tail : 1.0f - tail); // not x - x tail, which is NaN at infinity
     }
     else
     {

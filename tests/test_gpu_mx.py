@@ -702,3 +702,32 @@ def test_large_products_of_nothing(lib, O, T):
     y.fill_(GUARD)
     lib.mx_input_grad(0, lib.BF16, 0, 0, 0, 4, y.data_ptr(), lib.F32, O, 0, O, T, stream())
     assert not y.any()
+
+
+INF = float("inf")
+# f at +infinity and at -infinity: x * Phi(x) and x * sigmoid(x) have -infinity times 0 there
+AT_INFINITY = [(INF, 0.0), (1.0, 0.0), (1.0, -1.0), (INF, np.nan), (INF, np.nan)]
+
+
+@pytest.mark.parametrize("act", range(5))
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_activation_of_infinities(lib, t, act, pad):
+    """What an overflowed product feeds the layer: f at both infinities, and next to them values that are not touched by it."""
+    x = np.full((4, 64), 0.5)
+    x[0, 5], x[1, 40], x[2, 0], x[2, 63], x[3, 20] = INF, -INF, INF, -INF, np.nan
+    _, d, _ = place(torch.from_numpy(x), t, pad)
+    flat, y = room(4, 64, t, pad)
+    codes = torch.zeros(lib.mx_code_bytes(64, 4, 8), dtype=torch.uint8, device=DEV)
+    scales = torch.zeros(lib.mx_scale_bytes(64, 4), dtype=torch.uint8, device=DEV)
+    lib.mx_act_forward(d.data_ptr(), code(lib, t), 64 + pad, act, y.data_ptr(), 64 + pad, codes.data_ptr(), scales.data_ptr(), 64, 4, stream())
+    got = y.double().cpu().numpy()
+    high, low = AT_INFINITY[act]
+    assert np.array_equal([got[0, 5], got[2, 0]], [high, high])
+    assert np.array_equal([got[1, 40], got[2, 63]], [low, low], equal_nan=True)
+    assert np.isnan(got[3, 20])
+    # 0.5: as in test_activation
+    want = f64(np.array([0.5]), act)[0][0]
+    fine = x == 0.5
+    assert (np.abs(got - want)[fine] <= 12 * 2.0 ** -24 * 1.5 + torch.finfo(TYPES[t]).eps / 2 * abs(want)).all()
+    untouched(flat, y, pad, 0)
