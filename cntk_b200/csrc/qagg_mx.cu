@@ -272,13 +272,20 @@ struct BlockDecoder
 };
 
 // ---- pointwise functions -----------------------------------------------------------------------------------------------------
-// In fp32 whatever the type, within about 1e-7 * (1 + |x|): with the hardware's exponential and reciprocal, whose errors of a few
-// units of 2^-23 apply to e = exp(-|x|) <= 1, so that no form here overflows or cancels.  With expf, erff and IEEE divisions the
-// kernels were bound by their instructions: gelu of 4096 x 8192 bf16 took 53 us forward and 66 backward for 26 us of HBM traffic each.
+// In fp32 whatever the type, from the hardware's exponential and reciprocal, whose errors of one or two units of 2^-23 apply to
+// e = exp(-|x|) <= 1 and 1 / (1 + e), so that no form here overflows or cancels.  With 16-bit types the exponential's argument is rounded as
+// it comes, which is small beside half a step of the type.  fp32 results are good to a few units of the result itself, subnormal ones
+// included: there the argument's roundings are made up for.  With expf, normcdff and IEEE quotients the kernels were bound by
+// their instructions: gelu of 4096 x 8192 bf16 took 53 us forward and 66 backward for 26 us of HBM traffic each (now 36 and 38), of fp32 88
+// and 100 for 46 (now 61 and 64).
+template <class T>
 __device__ __forceinline__ float exp2_approx(float x)
 {
     float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    if constexpr (sizeof(T) == 4)
+        asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    else
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 __device__ __forceinline__ float rcp_approx(float x)
@@ -287,23 +294,71 @@ __device__ __forceinline__ float rcp_approx(float x)
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// exp(-k |x|)
+// the smaller of |x| and a limit beyond which exponentials are 0; NaN stays
+__device__ __forceinline__ float magnitude_to(float x, float limit)
+{
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(x)), "f"(limit));
+    return r;
+}
+// log2(e) in two floats
+constexpr float LOG2E = 1.44269502f, LOG2E_REST = 1.92596299e-8f, LN2 = 0.693147182f;
+// exp(-k |x|), k = 1 or 2
+template <class T>
 __device__ __forceinline__ float exp_minus(float k, float x)
 {
-    return exp2_approx(fabsf(x) * (-1.4426950408889634f * k));
+    if constexpr (sizeof(T) == 4)
+    {
+        // 2^(high + low) = 2^high + 2^high low ln 2, low being what the first product's rounding left
+        const float a = magnitude_to(x, 128.0f) * k, high = a * -LOG2E;
+        const float low = __fmaf_rn(a, -LOG2E_REST, __fmaf_rn(a, -LOG2E, -high)), e = exp2_approx<T>(high);
+        return __fmaf_rn(e * LN2, low, e);
+    }
+    else
+        return exp2_approx<T>(fabsf(x) * (-LOG2E * k));
 }
 
 // Phi(-|x|), the normal distribution's lower tail, and e = exp(-x^2 / 2): erfc(z) = (a1 t + ... + a5 t^5) exp(-z^2), t = 1 / (1 + p z), off by at
 // most 1.5e-7 (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26), at z = |x| / sqrt(2); its half.
+// fp32: the same form with nine terms, fitted to Phi(-x) exp(x^2 / 2) for the least largest relative error over x = 0 .. 14.5, 3.4e-8.
+template <class T>
 __device__ __forceinline__ float normal_tail(float x, float& e)
 {
-    const float t = rcp_approx(__fmaf_rn(0.3275911f * 0.70710678118654752f, fabsf(x), 1.0f));
-    e = exp2_approx(x * x * (-0.5f * 1.4426950408889634f));
-    float p = __fmaf_rn(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
-    p = __fmaf_rn(p, t, 0.5f * 1.421413741f);
-    p = __fmaf_rn(p, t, 0.5f * -0.284496736f);
-    p = __fmaf_rn(p, t, 0.5f * 0.254829592f);
-    return p * t * e;
+    if constexpr (sizeof(T) == 4)
+    {
+        const float a = magnitude_to(x, 16.0f), s = a * a, high = s * (-0.5f * LOG2E);
+        float low = __fmaf_rn(s, -0.5f * LOG2E_REST, __fmaf_rn(s, -0.5f * LOG2E, -high));
+        low = __fmaf_rn(__fmaf_rn(a, a, -s), -0.5f * LOG2E, low); // and what the square's left
+        e = exp2_approx<T>(high);
+        e = __fmaf_rn(e * LN2, low, e);
+        const float t = rcp_approx(__fmaf_rn(0.34f, a, 1.0f));
+        float p = __fmaf_rn(-0.0258764457f, t, 0.138357103f);
+        p = __fmaf_rn(p, t, -0.270871073f);
+        p = __fmaf_rn(p, t, 0.199717611f);
+        p = __fmaf_rn(p, t, -0.0431062728f);
+        p = __fmaf_rn(p, t, 0.114713587f);
+        p = __fmaf_rn(p, t, 0.115351707f);
+        p = __fmaf_rn(p, t, 0.136092231f);
+        p = __fmaf_rn(p, t, 0.135621578f);
+        return p * t * e;
+    }
+    else
+    {
+        const float t = rcp_approx(__fmaf_rn(0.3275911f * 0.70710678118654752f, fabsf(x), 1.0f));
+        e = exp2_approx<T>(x * x * (-0.5f * LOG2E));
+        float p = __fmaf_rn(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+        p = __fmaf_rn(p, t, 0.5f * 1.421413741f);
+        p = __fmaf_rn(p, t, 0.5f * -0.284496736f);
+        p = __fmaf_rn(p, t, 0.5f * 0.254829592f);
+        return p * t * e;
+    }
+}
+// Phi(x)
+template <class T>
+__device__ __forceinline__ float normal(float x, float& e)
+{
+    const float tail = normal_tail<T>(x, e);
+    return x < 0.0f ? tail : 1.0f - tail;
 }
 
 template <int ACT, class T>
@@ -314,10 +369,10 @@ __device__ __forceinline__ float act_value(float x)
     else if constexpr (ACT == QAGG_ACT_TANH)
     {
         if constexpr (sizeof(T) == 4)
-            return tanhf(x); // relative precision near 0
+            return tanhf(x);
         else
         {
-            const float e = exp_minus(2.0f, x);
+            const float e = exp_minus<T>(2.0f, x);
             const float t = (1.0f - e) * rcp_approx(1.0f + e);
             return fabsf(x) < 0.02f ? __fmaf_rn(x * x * x, -0.33333333f, x) : copysignf(t, x);
         }
@@ -325,18 +380,17 @@ __device__ __forceinline__ float act_value(float x)
     else if constexpr (ACT == QAGG_ACT_GELU)
     {
         float e;
-        const float tail = normal_tail(x, e);
-        return x * (x < 0.0f ? tail : 1.0f - tail); // not x - x tail, which is NaN at infinity
+        return x * normal<T>(x, e); // not x - x Phi(-x), which is NaN at infinity
     }
     else
     {
-        const float e = exp_minus(1.0f, x), r = rcp_approx(1.0f + e);
-        const float s = x < 0.0f ? e * r : r; // the sigmoid of x
+        const float e = exp_minus<T>(1.0f, x);
+        const float r = rcp_approx(1.0f + e), s = x < 0.0f ? e * r : r; // the sigmoid of x
         return ACT == QAGG_ACT_SIGMOID ? s : x * s;
     }
 }
 // derivative
-template <int ACT>
+template <int ACT, class T>
 __device__ __forceinline__ float act_slope(float x)
 {
     if constexpr (ACT == QAGG_ACT_RELU)
@@ -344,13 +398,12 @@ __device__ __forceinline__ float act_slope(float x)
     else if constexpr (ACT == QAGG_ACT_GELU)
     {
         float e;
-        const float tail = normal_tail(x, e);
-        return __fmaf_rn(x * 0.39894228040143268f, e, x < 0.0f ? tail : 1.0f - tail);
+        const float c = normal<T>(x, e);
+        return __fmaf_rn(x * 0.39894228040143268f, e, c);
     }
     else
     {
-        const float e = exp_minus(ACT == QAGG_ACT_TANH ? 2.0f : 1.0f, x);
-        const float r = rcp_approx(1.0f + e);
+        const float e = exp_minus<T>(ACT == QAGG_ACT_TANH ? 2.0f : 1.0f, x), r = rcp_approx(1.0f + e);
         const float d = e * r * r; // s (1 - s), s the sigmoid of |x| (tanh: of 2 |x|)
         if constexpr (ACT == QAGG_ACT_SIGMOID)
             return d;
@@ -669,7 +722,7 @@ __global__ void __launch_bounds__(MXT, (ACT >= 0 ? 5 : 4)) k_mx_unquantize(const
                 unpack32<T>(raw[p], g);
 #pragma unroll
                 for (int i = 0; i < S::V; ++i)
-                    v[i] = g[i] * act_slope<ACT>(v[i]);
+                    v[i] = g[i] * act_slope<ACT, T>(v[i]);
             }
             T* at = po + p * S::COLS * ldout;
             if (vecOut)

@@ -731,3 +731,43 @@ def test_activation_of_infinities(lib, t, act, pad):
     fine = x == 0.5
     assert (np.abs(got - want)[fine] <= 12 * 2.0 ** -24 * 1.5 + torch.finfo(TYPES[t]).eps / 2 * abs(want)).all()
     untouched(flat, y, pad, 0)
+
+
+def sweep(lo, hi, n):
+    """[columns, 32]: magnitudes from lo to hi, their logarithms evenly spread, both signs."""
+    v = np.exp(np.linspace(np.log(lo), np.log(hi), n))
+    return np.concatenate([v, -v]).reshape(-1, 32)
+
+
+@pytest.mark.parametrize("act", range(1, 5))
+def test_functions_in_fp32_keep_their_relative_precision(lib, act):
+    """fp32 in, fp32 out: a few units (of 2^-23) of the result itself, tails of the sigmoid and of GELU included.
+
+    An exponential is good to 3 units (the hardware's 2, its argument's rest put back), a reciprocal to 1, sums and products to half a unit.
+    Sigmoid and SiLU: 3, 1 + e and its reciprocal 1.5, two products 1.  Slopes of sigmoid and tanh: 3, twice 1.5, two products 1: 7.  tanh
+    itself: 2.  GELU: t = 1 / (1 + c x) is off by 1.5 units, which the tail's form makes 3.6 of, its polynomial's fit and steps 2, the
+    exponential 3, three products 1.5: 10.  Slopes of GELU and SiLU: sums of two terms, each as good as that."""
+    x = sweep(1e-30, 88.0, 4096).astype(np.float32)
+    n = x.shape[0]
+    d = torch.from_numpy(x).to(DEV)
+    y, dx = torch.zeros_like(d), torch.ones_like(d)
+    codes = torch.zeros(lib.mx_code_bytes(32, n, 8), dtype=torch.uint8, device=DEV)
+    scales = torch.zeros(lib.mx_scale_bytes(32, n), dtype=torch.uint8, device=DEV)
+    lib.mx_act_forward(d.data_ptr(), lib.F32, 32, act, y.data_ptr(), 32, codes.data_ptr(), scales.data_ptr(), 32, n, stream())
+    lib.mx_act_backward(dx.data_ptr(), lib.F32, 32, codes.data_ptr(), scales.data_ptr(), act, dx.data_ptr(), 32, 32, n, stream())
+    unit, least = 2.0 ** -23, 8 * 2.0 ** -149  # subnormal factors and results: roundings of the smallest step
+    units = 10 if act == 3 else 7
+    want = f64(x.astype(np.float64), act)[0]
+    err = np.abs(y.double().cpu().numpy() - want)
+    assert (err <= units * unit * np.abs(want) + least * (np.abs(x) + 1)).all(), f"worst {np.max(err / (unit * np.abs(want) + least))} units"
+    kept = mx_util.values(x, 8)
+    want = f64(kept, act)[1]
+    s = torch.sigmoid(torch.from_numpy(kept)).numpy()
+    if act == 3:
+        size = 0.5 * torch.special.erfc(-torch.from_numpy(kept) / 2 ** 0.5).numpy() + 0.4 * np.abs(kept) * np.exp(-kept ** 2 / 2)
+    elif act == 4:
+        size = s + np.abs(kept) * s * torch.sigmoid(-torch.from_numpy(kept)).numpy()
+    else:
+        size = np.abs(want)
+    err = np.abs(dx.double().cpu().numpy() - want)
+    assert (err <= units * unit * size + least * (np.abs(kept) + 1)).all(), f"worst {np.max(err / (unit * size + least))} units"
