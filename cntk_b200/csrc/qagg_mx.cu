@@ -276,7 +276,7 @@ struct BlockDecoder
 // e = exp(-|x|) <= 1 and 1 / (1 + e), so that no form here overflows or cancels.  With 16-bit types the exponential's argument is rounded as
 // it comes, which is small beside half a step of the type.  fp32 results are good to a few units of the result itself, subnormal ones
 // included: there the argument's roundings are made up for.  With expf, normcdff and IEEE quotients the kernels were bound by
-// their instructions: gelu of 4096 x 8192 bf16 took 53 us forward and 66 backward for 26 us of HBM traffic each (now 36 and 38), of fp32 88
+// their instructions: gelu of 4096 x 8192 bf16 took 53 us forward and 66 backward for 26 us of HBM traffic each (now 37 and 38), of fp32 88
 // and 100 for 46 (now 61 and 64).
 template <class T>
 __device__ __forceinline__ float exp2_approx(float x)
@@ -318,9 +318,10 @@ __device__ __forceinline__ float exp_minus(float k, float x)
         return exp2_approx<T>(fabsf(x) * (-LOG2E * k));
 }
 
-// Phi(-|x|), the normal distribution's lower tail, and e = exp(-x^2 / 2): erfc(z) = (a1 t + ... + a5 t^5) exp(-z^2), t = 1 / (1 + p z), off by at
-// most 1.5e-7 (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26), at z = |x| / sqrt(2); its half.
-// fp32: the same form with nine terms, fitted to Phi(-x) exp(x^2 / 2) for the least largest relative error over x = 0 .. 14.5, 3.4e-8.
+// Phi(-|x|), the normal distribution's lower tail, and e = exp(-x^2 / 2), as (a1 t + a2 t^2 + ...) e, t = 1 / (1 + c |x|): the form of Abramowitz
+// and Stegun, Handbook of Mathematical Functions, 7.1.26, whose own five terms are good to 1.5e-7 of 1 but to 2e-3 of the tail at 5.
+// 16-bit types: six terms, within 2.4e-7 near 0 and 2.4e-5 of the tail everywhere (half a step of fp16 is 4.9e-4).  fp32: nine terms,
+// fitted for the least largest relative error over |x| = 0 .. 14.5, 3.4e-8.
 template <class T>
 __device__ __forceinline__ float normal_tail(float x, float& e)
 {
@@ -344,12 +345,13 @@ __device__ __forceinline__ float normal_tail(float x, float& e)
     }
     else
     {
-        const float t = rcp_approx(__fmaf_rn(0.3275911f * 0.70710678118654752f, fabsf(x), 1.0f));
+        const float t = rcp_approx(__fmaf_rn(0.296f, fabsf(x), 1.0f));
         e = exp2_approx<T>(x * x * (-0.5f * LOG2E));
-        float p = __fmaf_rn(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
-        p = __fmaf_rn(p, t, 0.5f * 1.421413741f);
-        p = __fmaf_rn(p, t, 0.5f * -0.284496736f);
-        p = __fmaf_rn(p, t, 0.5f * 0.254829592f);
+        float p = __fmaf_rn(-0.0822813883f, t, 0.243228272f);
+        p = __fmaf_rn(p, t, -0.045148883f);
+        p = __fmaf_rn(p, t, 0.156217799f);
+        p = __fmaf_rn(p, t, 0.109275274f);
+        p = __fmaf_rn(p, t, 0.118709125f);
         return p * t * e;
     }
 }

@@ -406,7 +406,8 @@ int qagg_mx_input_grad(void* stream, const void* dy, int dy_type, int64_t ld_dy,
  * dx = dy * f'(x as kept).  y may be x, dx may be dy (same ld).  QAGG_ACT_GELU is x * Phi(x), QAGG_ACT_SILU x * sigmoid(x); the slope of
  * QAGG_ACT_RELU at 0 (also at values that were rounded to 0) is 0.  Infinite x are taken as the formulas have it: relu, GELU and SiLU of
  * infinity are infinity, and GELU and SiLU of -infinity, which is -infinity times 0, are NaN.  A kept block with a NaN or an infinity
- * gives NaN gradients.  With fp32 f is good to ten units in the last place, tails included, f' to as much of its largest term. */
+ * gives NaN gradients.  With fp32 f is good to ten units in the last place, tails included, f' to as much of its largest term;
+ * with 16-bit types both are rounded from values good to 2^-14, except that exponentials below 2^-126 count as 0. */
 #define QAGG_ACT_RELU 0
 #define QAGG_ACT_SIGMOID 1
 #define QAGG_ACT_TANH 2

@@ -771,3 +771,37 @@ def test_functions_in_fp32_keep_their_relative_precision(lib, act):
         size = np.abs(want)
     err = np.abs(dx.double().cpu().numpy() - want)
     assert (err <= units * unit * size + least * (np.abs(kept) + 1)).all(), f"worst {np.max(err / (unit * size + least))} units"
+
+
+@pytest.mark.parametrize("act", range(5))
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_functions_in_half_precision_are_rounded_once(lib, t, act):
+    """16-bit results: half a step of the value itself, tails included, and what fp32 loses before that rounding.
+
+    exp(-x^2 / 2) and exp(-|x|) with the hardware's exponential: its argument, up to 126 powers of two, is rounded twice (2^-24 each, times
+    126 ln 2: 2^-17 of the result), itself within 2^-22; the polynomial of GELU's tail within 2.5e-5; tanh from 0.02 on loses
+    1 / 0.04 of 2^-22 to a difference.  Together below 2^-14.  Exponentials below 2^-126 are 0, and with them results below that times |x|."""
+    x = torch.from_numpy(sweep(1e-4, 88.0, 8192)).to(TYPES[t])
+    n = x.shape[0]
+    d = x.to(DEV)
+    x = x.double().numpy()
+    y, dx = torch.zeros_like(d), torch.ones_like(d)
+    codes = torch.zeros(lib.mx_code_bytes(32, n, 8), dtype=torch.uint8, device=DEV)
+    scales = torch.zeros(lib.mx_scale_bytes(32, n), dtype=torch.uint8, device=DEV)
+    lib.mx_act_forward(d.data_ptr(), code(lib, t), 32, act, y.data_ptr(), 32, codes.data_ptr(), scales.data_ptr(), 32, n, stream())
+    lib.mx_act_backward(dx.data_ptr(), code(lib, t), 32, codes.data_ptr(), scales.data_ptr(), act, dx.data_ptr(), 32, 32, n, stream())
+    eps = torch.finfo(TYPES[t]).eps
+    kept = mx_util.values(x, 8)
+    s = torch.sigmoid(torch.from_numpy(kept)).numpy()
+    want = f64(kept, act)[1]
+    terms = np.abs(want)  # of a slope that is a sum: the terms' magnitudes
+    if act == 3:
+        terms = 0.5 * torch.special.erfc(-torch.from_numpy(kept) / 2 ** 0.5).numpy() + 0.4 * np.abs(kept) * np.exp(-kept ** 2 / 2)
+    if act == 4:
+        terms = s + np.abs(kept) * s * torch.sigmoid(-torch.from_numpy(kept)).numpy()
+    for got, ref, size, at in ((y, f64(x, act)[0], None, x), (dx, want, terms, kept)):
+        size = np.abs(ref) if size is None else size
+        least = (2.0 ** -25 if t == "f16" else 0) + 2.0 ** -126 * (np.abs(at) + 1)
+        err = np.abs(got.double().cpu().numpy() - ref)
+        tol = eps / 2 * np.abs(ref) + 2.0 ** -14 * size * (1 + eps) + least
+        assert (err <= tol).all(), f"worst {np.max(err / tol)}, at {np.argmax(err / tol)}"
