@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
     const int resultWarps = bn > 128 ? 8 : 4;
     const int bufs = bn > 128 ? 1 : 2; // accumulators, 128 columns apart
     constexpr unsigned SIDE = 256;     // block scales: 24 columns a stage
-    constexpr int CHAIN_STEPS = (sizeof(T) != 4 ? CHAIN_16BIT : ACC == 128 ? CHAIN_SINGLE : CHAIN) / 4;
+    const int chainSteps = (sizeof(T) != 4 ? CHAIN_16BIT : bufs == 1 ? CHAIN_SINGLE : CHAIN) / 4;
 
     // The copying thread's time per step counts: what depends on the tile alone is worked out once per tile.
     struct Source
@@ -533,7 +533,7 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
                     else
                         tc_commit(&bars.empty[ring.s]);
                     ring.next(S);
-                    if (++inChain == CHAIN_STEPS || i + 1 == count)
+                    if (++inChain == chainSteps || i + 1 == count)
                     {
                         if constexpr (PAIR)
                             tc_commit_pair(&bars.ready[chain.buf]);
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
                 const long long m0 = (long long) (tile % a.tilesM) * (PAIR ? 256 : 128) + (PAIR ? rank * 128 : 0), n0 = (long long) (tile / a.tilesM) * bn;
                 const float bias = a.bias && a.splits == 1 && m0 + m < a.O ? a.bias[m0 + m] : 0.0f;
                 float* buf = reinterpret_cast<float*>(stage0);
-                if (!PAIR && a.tiles <= tileStep && count <= CHAIN_STEPS)
+                if (!PAIR && a.tiles <= tileStep && count <= chainSteps)
                 {
                     drain_chain(&bars, mine, cols, count == 0, [&](int j, const float(&v)[16]) {
                         if (a.splits > 1)
@@ -589,7 +589,7 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
 #pragma unroll
                 for (int j = 0; j < ACC; ++j)
                     acc[j] = 0.0f;
-                for (int i = 0; i < count; i += CHAIN_STEPS, chain.next(bufs))
+                for (int i = 0; i < count; i += chainSteps, chain.next(bufs))
                     take_chain<PAIR>(&bars, chain.buf, chain.par, mine + chain.buf * 128, cols, i == 0, acc);
                 if (!PAIR && a.splits > 1)
                     put_partial<false>(buf, bn, m, half * 128, cols, acc);

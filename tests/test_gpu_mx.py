@@ -805,3 +805,36 @@ def test_functions_in_half_precision_are_rounded_once(lib, t, act):
         err = np.abs(got.double().cpu().numpy() - ref)
         tol = eps / 2 * np.abs(ref) + 2.0 ** -14 * size * (1 + eps) + least
         assert (err <= tol).all(), f"worst {np.max(err / tol)}, at {np.argmax(err / tol)}"
+
+
+# ---- how much a long sum may lose ---------------------------------------------------------------------------------------------
+# The tensor cores truncate the running sum to fp32.  The worst case: 1 first, then instructions whose products add up to 3/4 of the
+# sum's unit in the last place, 2^-23, all of which the truncation drops.  A chain of n instructions loses 3/4 n units that way; the chains
+# after it hold multiples of 3/4 unit of their own and lose nothing, and n being a multiple of 4 they are added exactly.
+UNIT = 2.0 ** -23
+
+
+def ones(lib, m, n, fmt):
+    """A packed m x n matrix of ones."""
+    x = torch.ones(n, m, dtype=torch.bfloat16, device=DEV)
+    return quantized(lib, x, m, n, m, "bf16", fmt)
+
+
+def lost(out, want):
+    """Least and most of what is missing from `want`, in units of 2^-23."""
+    return (want - float(out.max())) / UNIT, (want - float(out.min())) / UNIT
+
+
+@pytest.mark.parametrize("O,T,K", [(128, 16, 131072), (128, 48, 131072), (128, 100, 131072), (200, 250, 131072), (4096, 2304, 16384)])
+def test_long_sums_of_the_product(lib, O, T, K):
+    """64 products an instruction; 32 instructions to a chain, 64 where a tile is 256 wide (more than 128 tokens)."""
+    w = torch.full((K, O), 0.75 * UNIT / 64, device=DEV)  # O x K
+    w[0] = 1.0
+    w[1:32] = 0.0  # they share a scale with the 1
+    wc, ws = quantized(lib, w, O, K, O, "f32", lib.MXFP4, True)
+    xc, xs = ones(lib, K, T, lib.MXFP4)
+    y = torch.zeros(T, O, device=DEV)
+    lib.mx_times(wc.data_ptr(), ws.data_ptr(), xc.data_ptr(), xs.data_ptr(), 0, y.data_ptr(), lib.F32, O, O, T, K, stream())
+    lib.mx_check(stream())
+    least, most = lost(y, 1.0 + (K - 32) * 0.75 * UNIT / 64)
+    assert least >= 0 and most <= 0.75 * (32 if T <= 128 else 64)
