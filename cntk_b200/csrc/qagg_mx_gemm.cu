@@ -13,8 +13,8 @@
 // the last place, 6.8e-6 of the result after 512 of them.  So where the output is fp32 a chain ends after CHAIN instructions; the
 // result warps add its value to their registers (round to nearest) and hand the accumulator back, which takes about 2000 cycles
 // from the last product to the next.  Two accumulators in turn hide that, and the next tile begins while this one is being
-// written.  (A 256-wide tile of the 4-bit product has room for one.)  For 16-bit outputs, which round 300 times more coarsely, a
-// chain is CHAIN_16BIT instructions.
+// written.  (A 256-wide tile of the 4-bit product has room for one.)
+// 16-bit outputs, which round more coarsely, have longer chains.
 //
 // Where there are fewer tiles than SMs the contraction is split over the CTAs of a cluster, whose partial sums are added through
 // distributed shared memory in rank order: no workspace, no atomics, the same bits on every run.
@@ -40,8 +40,11 @@ constexpr int GEMM_SMEM_MAX = 224 * 1024; // dynamic; barriers and scales take a
 // barriers.
 constexpr int GEMM_SMEM_MIN = 200 * 1024;
 // Tensor-core instructions in a row on one accumulator.  After 32 the sums are within 3e-7; with a single accumulator, where every
-// chain costs its hand-over, 64 are taken: within 6e-7, as a sum in plain fp32 is.
-constexpr int CHAIN = 32, CHAIN_SINGLE = 64, CHAIN_16BIT = 1024;
+// chain costs its hand-over, 64 are taken: within 6e-7, as a sum in plain fp32 is.  n instructions lose less than n units of 2^-23.  A
+// 16-bit result's own rounding is half a step: 4096 such units for fp16, 32768 for bf16; chains for them lose a 32nd of that at most.
+constexpr int CHAIN = 32, CHAIN_SINGLE = 64, CHAIN_FP16 = 128, CHAIN_BF16 = 1024;
+template <class T, bool SINGLE>
+constexpr int CHAIN_OF = std::is_same_v<T, __half> ? CHAIN_FP16 : std::is_same_v<T, __nv_bfloat16> ? CHAIN_BF16 : SINGLE ? CHAIN_SINGLE : CHAIN;
 
 struct GemmBars
 {
@@ -404,7 +407,7 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
     const int resultWarps = bn > 128 ? 8 : 4;
     const int bufs = bn > 128 ? 1 : 2; // accumulators, 128 columns apart
     constexpr unsigned SIDE = 256;     // block scales: 24 columns a stage
-    const int chainSteps = (sizeof(T) != 4 ? CHAIN_16BIT : bufs == 1 ? CHAIN_SINGLE : CHAIN) / 4;
+    const int chainSteps = (bufs == 1 ? CHAIN_OF<T, true> : CHAIN_OF<T, false>) / 4;
 
     // The copying thread's time per step counts: what depends on the tile alone is worked out once per tile.
     struct Source
@@ -896,7 +899,7 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
 {
     using G = GradGroups<(DENSE > 0), PAIR>;
     constexpr int NP = DENSE ? DENSE : 1;
-    constexpr int CHAIN_STEPS = (sizeof(TO) != 4 ? CHAIN_16BIT : G::accumulators == 1 ? CHAIN_SINGLE : CHAIN) / 4 / NP;
+    constexpr int CHAIN_STEPS = CHAIN_OF<TO, G::accumulators == 1> / 4 / NP;
     constexpr int WIDEST = G::widest, SLOTS = G::slots, BUFS = G::accumulators;
     extern __shared__ unsigned char dyn[];
     __shared__ GemmBars bars;

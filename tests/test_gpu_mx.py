@@ -838,3 +838,39 @@ def test_long_sums_of_the_product(lib, O, T, K):
     lib.mx_check(stream())
     least, most = lost(y, 1.0 + (K - 32) * 0.75 * UNIT / 64)
     assert least >= 0 and most <= 0.75 * (32 if T <= 128 else 64)
+
+
+def test_sums_for_fp16_results(lib):
+    """A chain for an fp16 result has 128 instructions at most, and loses 96 of the 8192 units of 2^-23 that fp16's step at 1 has.  The
+    sums here lie 150 or more units above the middle between two fp16 values, those of a chain four times as long would lie below it."""
+    tie, small = 1.0 + 2.0 ** -11, 0.75 * UNIT
+    step = 2.0 ** -10
+
+    # dx: 16 products an instruction (and as many for the second plane of an fp16 dy, which is 0).  Splits take an eighth each.
+    for t, O in (("f16", 8 * 8192), ("bf16", 8 * 16384)):
+        I, T = 128, 64
+        w = torch.full((O, I), small / 16, device=DEV)
+        w[:16] = 0.0
+        w[0], w[1] = 1.0, 2.0 ** -11
+        wc, ws = quantized(lib, w, I, O, I, "f32", lib.MXFP4)
+        dy = torch.ones(T, O, dtype=TYPES[t], device=DEV)
+        dy[:, O // 8:] = 0.0  # one CTA's part
+        want = tie + (O // 8 - 16) * small / 16
+        assert want - tie > 150 * UNIT
+        dx = torch.zeros(T, I, dtype=torch.float16, device=DEV)
+        lib.mx_input_grad(dy.data_ptr(), code(lib, t), O, wc.data_ptr(), ws.data_ptr(), lib.MXFP4, dx.data_ptr(), lib.F16, I, O, I, T, stream())
+        lib.mx_check(stream())
+        assert bool((dx == 1.0 + step).all())
+
+    O, T, K = 128, 16, 8 * 65536  # 64 products an instruction
+    w = torch.full((K, O), small / 64, device=DEV)
+    w[:64] = 0.0
+    w[0], w[32] = 1.0, 2.0 ** -11
+    wc, ws = quantized(lib, w, O, K, O, "f32", lib.MXFP4, True)
+    x = torch.ones(T, K, device=DEV)
+    x[:, K // 8:] = 0.0
+    xc, xs = quantized(lib, x, K, T, K, "f32", lib.MXFP4)
+    y = torch.zeros(T, O, dtype=torch.float16, device=DEV)
+    lib.mx_times(wc.data_ptr(), ws.data_ptr(), xc.data_ptr(), xs.data_ptr(), 0, y.data_ptr(), lib.F16, O, O, T, K, stream())
+    lib.mx_check(stream())
+    assert bool((y == 1.0 + step).all())
