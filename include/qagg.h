@@ -370,8 +370,9 @@ int qagg_wait_flags(void* stream, const unsigned* flags_dev, int n, int skip, un
  *
  * Dense matrices are column-major with `ld` elements from one column to the next (ld >= rows), of type QAGG_F32, QAGG_F16 or
  * QAGG_BF16, aligned to their type.  bf16 operands whose base and ld are multiples of 16 bytes are the fast case of the products;
- * any other alignment, and fp16 and fp32, are taken too.  Results do not depend on alignment.  Elements between a column's
- * rows and its ld are neither read nor written.  Rows < 2^30, columns <= 65535 * 128 (the second dimension of a gradient product's
+ * any other alignment, and fp16 and fp32, are taken too.  Results do not depend on alignment, with one exception: a bf16 dy of the
+ * gradients in that fast case is summed in another order than elsewhere, and results differ in their last bits.  Elements between a
+ * column's rows and its ld are neither read nor written.  Rows < 2^30, columns <= 65535 * 128 (the second dimension of a gradient product's
  * result: 65535 * 64).  Sums and functions are computed in fp32 and rounded once to the output type.  All calls only enqueue
  * kernels on `stream` (they may be captured), allocate nothing and use no workspace: calls on different streams are independent.
  * As everywhere in this library the buffers and the stream belong to the current device. */

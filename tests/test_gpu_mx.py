@@ -874,3 +874,36 @@ def test_sums_for_fp16_results(lib):
     lib.mx_times(wc.data_ptr(), ws.data_ptr(), xc.data_ptr(), xs.data_ptr(), 0, y.data_ptr(), lib.F16, O, O, T, K, stream())
     lib.mx_check(stream())
     assert bool((y == 1.0 + step).all())
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_results_and_alignment(lib, t):
+    """Everything but the gradients of a bf16 dy has the same bits at every alignment; those agree within what their sums may lose."""
+    rng = np.random.default_rng(31)
+    O, I, T = 2304, 700, 1100
+    _, near, dy = dense(rng, T, O, t, 0, 0, 1e-2)
+    _, far, _ = place(torch.from_numpy(dy), t, 3, 1)
+    (xc, xs), x = packed(rng, T, I, mx_util.INT8)
+    (wc, ws), w = packed(rng, O, I, mx_util.FP4, 0.05)
+    results = []
+    for d, ld, pad, offset in ((near, O, 0, 0), (far, O + 3, 3, 1)):
+        flat, dw = room(I, O, "f32", 0, offset)
+        lib.mx_weight_grad(d.data_ptr(), code(lib, t), ld, xc.data_ptr(), xs.data_ptr(), 8, dw.data_ptr(), O, I, T, False, stream())
+        flat2, dx = room(T, I, t, pad, offset)
+        lib.mx_input_grad(d.data_ptr(), code(lib, t), ld, wc.data_ptr(), ws.data_ptr(), 4, dx.data_ptr(), code(lib, t), I + pad, O, I, T, stream())
+        codes, scales = run_quantize(lib, d, O, T, t, ld, 8, False)
+        turned, turnedScales = run_quantize(lib, d, O, T, t, ld, 4, True)
+        flat3, back = room(T, O, t, pad, offset)
+        lib.mx_unquantize(codes.data_ptr(), scales.data_ptr(), back.data_ptr(), code(lib, t), O + pad, O, T, 8, stream())
+        flat4, y = room(T, O, t, pad, offset)
+        x4 = to_dev(*mx_util.pack(x, 4))
+        lib.mx_times(wc.data_ptr(), ws.data_ptr(), x4[0].data_ptr(), x4[1].data_ptr(), 0, y.data_ptr(), code(lib, t), O + pad, O, T, I, stream())
+        torch.cuda.synchronize()
+        results.append([codes, scales, turned, turnedScales, back.clone(), y.clone(), dw.clone(), dx.clone()])
+    for k, (a, b) in enumerate(zip(*results)):
+        if t != "bf16" or k < 6:
+            assert torch.equal(a, b), k
+    for dw, dx in ((r[6], r[7]) for r in results):
+        planes = {"bf16": 1, "f16": 2, "f32": 3}[t]
+        check(dw, x.T @ dy, np.abs(x).T @ np.abs(dy), planes * T / 16, "f32", "weight gradient")
+        check(dx, dy @ w, np.abs(dy) @ np.abs(w), planes * O / 16, t, "input gradient")
