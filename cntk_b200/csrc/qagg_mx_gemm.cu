@@ -25,13 +25,31 @@
 #include <algorithm>
 #include <atomic>
 #include <cstring>
+#include <mutex>
 #include <string>
 #include <type_traits>
 
 namespace qagg {
 
-// set by a bounded wait that ran out; read and cleared by qagg_mx_check
-__device__ unsigned g_mxStatus;
+// set by a bounded wait that ran out; qagg_mx_check takes it, in one step, and reads what it took
+__device__ unsigned g_mxStatus, g_mxTaken;
+__global__ void k_mx_take_status()
+{
+    g_mxTaken = atomicExch(&g_mxStatus, 0u);
+}
+// A wait of the product kernels on a barrier that nothing completes, and one more behind it, which returns at once.
+__global__ void __launch_bounds__(32) k_mx_wait_selftest(unsigned long long limitNs)
+{
+    __shared__ unsigned long long bar;
+    __shared__ unsigned broken;
+    if (threadIdx.x == 0)
+    {
+        mbar_init(&bar, 1);
+        broken = 0;
+        tc_wait(&bar, 0, &broken, &g_mxStatus, limitNs);
+        tc_wait(&bar, 0, &broken, &g_mxStatus);
+    }
+}
 
 constexpr int MAX_STAGES = 8;
 constexpr int GEMM_SMEM_MAX = 224 * 1024; // dynamic; barriers and scales take a little more
@@ -1624,16 +1642,44 @@ int qagg_mx_input_grad(void* stream, const void* dy, int dy_type, int64_t ld_dy,
 
 int qagg_mx_check(void* stream)
 {
-    int rc = check_cuda(cudaStreamSynchronize((cudaStream_t) stream), "qagg_mx_check");
+    const cudaStream_t st = (cudaStream_t) stream;
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    int rc = check_cuda(cudaStreamIsCapturing(st, &capture), "qagg_mx_check");
+    if (rc)
+        return rc;
+    if (capture != cudaStreamCaptureStatusNone)
+        return fail(QAGG_ESTATE, "qagg_mx_check: the stream is being captured");
+    // another stream's capture, on this thread or another, is not to be disturbed by the calls below, which do not concern it
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    rc = check_cuda(cudaThreadExchangeStreamCaptureMode(&mode), "qagg_mx_check");
     if (rc)
         return rc;
     unsigned status = 0;
-    rc = check_cuda(cudaMemcpyFromSymbol(&status, g_mxStatus, sizeof(status)), "qagg_mx_check");
+    rc = check_cuda(cudaStreamSynchronize(st), "qagg_mx_check");
+    if (!rc)
+    {
+        static std::mutex one; // g_mxTaken is one word per device
+        const std::lock_guard<std::mutex> guard(one);
+        k_mx_take_status<<<1, 1, 0, st>>>();
+        cudaError_t e = cudaGetLastError();
+        if (e == cudaSuccess)
+            e = cudaMemcpyFromSymbolAsync(&status, g_mxTaken, sizeof(status), 0, cudaMemcpyDeviceToHost, st);
+        if (e == cudaSuccess)
+            e = cudaStreamSynchronize(st);
+        rc = check_cuda(e, "qagg_mx_check");
+    }
+    cudaThreadExchangeStreamCaptureMode(&mode);
     if (rc || !status)
         return rc;
-    const unsigned zero = 0;
-    rc = check_cuda(cudaMemcpyToSymbol(g_mxStatus, &zero, sizeof(zero)), "qagg_mx_check");
-    return rc ? rc : fail(QAGG_ETIMEOUT, "qagg_mx_check: a bounded wait inside a product kernel ran out; its results are invalid");
+    return fail(QAGG_ETIMEOUT, "qagg_mx_check: a bounded wait inside a product kernel ran out on this device; results since the last check may be invalid");
+}
+
+int qagg_mx_wait_selftest(void* stream, int64_t limit_ns)
+{
+    if (limit_ns < 1 || limit_ns > 1000000000)
+        return fail(QAGG_EINVAL, "qagg_mx_wait_selftest: the limit must be 1 .. 10^9 ns");
+    k_mx_wait_selftest<<<1, 32, 0, (cudaStream_t) stream>>>((unsigned long long) limit_ns);
+    return check_cuda(cudaGetLastError(), "product wait self-test launch");
 }
 
 } // extern "C"

@@ -37,7 +37,7 @@ __device__ __forceinline__ void mbar_arrive_remote(unsigned long long* bar, unsi
                  "r"(rank)
                  : "memory");
 }
-__device__ __forceinline__ void tc_wait(unsigned long long* bar, unsigned parity, unsigned* broken, unsigned* status)
+__device__ __forceinline__ void tc_wait(unsigned long long* bar, unsigned parity, unsigned* broken, unsigned* status, unsigned long long limitNs = TC_WAIT_NS)
 {
     if (mbar_suspend_wait(bar, parity))
         return;
@@ -46,7 +46,7 @@ __device__ __forceinline__ void tc_wait(unsigned long long* bar, unsigned parity
     {
         if (*reinterpret_cast<volatile unsigned*>(broken))
             return;
-        if (clock_ns() - began > TC_WAIT_NS)
+        if (clock_ns() - began > limitNs)
         {
             *reinterpret_cast<volatile unsigned*>(broken) = 1u;
             atomicOr(status, 1u);

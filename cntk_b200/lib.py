@@ -37,7 +37,7 @@ EXPORTS = [
     "qagg_agg_f64_create", "qagg_agg_f64_step", "qagg_agg_f64_step_group", "qagg_agg_f64_reset_residuals", "qagg_agg_f64_residuals",
     "qagg_agg_f64_destroy", "qagg_agg_f64_copy_residual", "qagg_dense_set_fp16",
     "qagg_mx_code_bytes", "qagg_mx_scale_bytes", "qagg_mx_quantize", "qagg_mx_unquantize", "qagg_mx_times", "qagg_mx_weight_grad", "qagg_mx_input_grad",
-    "qagg_mx_act_forward", "qagg_mx_act_backward", "qagg_mx_check",
+    "qagg_mx_act_forward", "qagg_mx_act_backward", "qagg_mx_check", "qagg_mx_wait_selftest",
 ]
 
 
@@ -157,6 +157,7 @@ _lib.qagg_mx_input_grad.argtypes = [c_vp, c_vp, c_int, c_i64, c_vp, c_vp, c_int,
 _lib.qagg_mx_act_forward.argtypes = [c_vp, c_vp, c_int, c_i64, c_int, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64]
 _lib.qagg_mx_act_backward.argtypes = [c_vp, c_vp, c_int, c_i64, c_vp, c_vp, c_int, c_vp, c_i64, c_i64, c_i64]
 _lib.qagg_mx_check.argtypes = [c_vp]
+_lib.qagg_mx_wait_selftest.argtypes = [c_vp, c_i64]
 
 
 def raw():
@@ -301,8 +302,13 @@ def mx_act_backward(dy_ptr, dtype, ld_dy, codes_ptr, scales_ptr, act, dx_ptr, ld
 
 
 def mx_check(stream=0):
-    """Waits for the stream and raises if a bounded wait inside a product kernel ran out since the last call."""
+    """Waits for the stream and raises if a bounded wait inside a product kernel ran out on the device since the last call."""
     _ok(_lib.qagg_mx_check(stream))
+
+
+def mx_wait_selftest(limit_ns, stream=0):
+    """A bounded wait that nothing ends: the next mx_check raises."""
+    _ok(_lib.qagg_mx_wait_selftest(stream, limit_ns))
 
 
 class Plan:

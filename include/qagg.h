@@ -416,9 +416,15 @@ int qagg_mx_input_grad(void* stream, const void* dy, int dy_type, int64_t ld_dy,
 #define QAGG_ACT_SILU 4
 int qagg_mx_act_forward(void* stream, const void* x, int type, int64_t ld_x, int act, void* y, int64_t ld_y, void* codes, void* scales, int64_t M, int64_t N);
 int qagg_mx_act_backward(void* stream, const void* dy, int type, int64_t ld_dy, const void* codes, const void* scales, int act, void* dx, int64_t ld_dx, int64_t M, int64_t N);
-/* Waits for `stream`; QAGG_ETIMEOUT if a bounded wait inside a product kernel ran out since the last call (never observed), and
- * clears that report. */
+/* Every wait inside the product kernels is bounded: 4 s for one step of a ring or one chain.  One that runs out (never observed) ends its
+ * kernel, whose results are then invalid, and is noted in a word of the device.  qagg_mx_check waits for `stream` and returns
+ * QAGG_ETIMEOUT if the word is set, clearing it: the report covers all streams and callers of the device since the last check, and
+ * one of them gets it.  Call it where results are read, as with qagg_agg_check.  It touches no other stream and no capture; a stream that is
+ * being captured is refused (QAGG_ESTATE).
+ * qagg_mx_wait_selftest runs one such wait on a barrier that nothing completes and that gives up after limit_ns (1 .. 10^9): the next
+ * check reports it. */
 int qagg_mx_check(void* stream);
+int qagg_mx_wait_selftest(void* stream, int64_t limit_ns);
 
 /* Per-phase device timing of the steps that follow (no reference counterpart; the reference only has the wall-clock
  * "Actual gradient aggregation time" trace, AllReduceDistGradAggregator.h:241-246, 560-565).  When enabled, each step records

@@ -907,3 +907,64 @@ def test_results_and_alignment(lib, t):
         planes = {"bf16": 1, "f16": 2, "f32": 3}[t]
         check(dw, x.T @ dy, np.abs(x).T @ np.abs(dy), planes * T / 16, "f32", "weight gradient")
         check(dx, dy @ w, np.abs(dy) @ np.abs(w), planes * O / 16, t, "input gradient")
+
+
+def test_a_wait_that_runs_out_is_reported(lib):
+    """A bounded wait on a barrier that nothing completes, with a limit of 20 ms: the kernel ends, the next check says so, once."""
+    lib.mx_check(stream())
+    lib.mx_wait_selftest(20_000_000, stream())
+    with pytest.raises(lib.QaggError) as e:
+        lib.mx_check(stream())
+    assert "error -5" in str(e.value)
+    lib.mx_check(stream())
+    # the report is the device's: a check of any stream brings it, after that stream's work
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    lib.mx_wait_selftest(1_000_000, a.cuda_stream)
+    a.synchronize()
+    with pytest.raises(lib.QaggError):
+        lib.mx_check(b.cuda_stream)
+    lib.mx_check(a.cuda_stream)
+
+
+def test_checks_from_several_threads_report_once(lib):
+    """Eight threads check at the same time: one of them gets the report."""
+    import threading
+    for _ in range(10):
+        lib.mx_wait_selftest(1000, stream())
+        torch.cuda.synchronize()
+        streams, got = [torch.cuda.Stream() for _ in range(8)], []
+
+        def look(s):
+            torch.cuda.set_device(0)
+            try:
+                lib.mx_check(s.cuda_stream)
+            except lib.QaggError as e:
+                got.append(str(e))
+
+        threads = [threading.Thread(target=look, args=(s,)) for s in streams]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert len(got) == 1 and "error -5" in got[0], got
+    lib.mx_check(stream())
+
+
+def test_check_beside_a_capture(lib):
+    """While a stream is being captured another one can be checked; the captured one is refused, and the capture goes on."""
+    x = torch.randn(64, 128, device=DEV)
+    codes = torch.zeros(lib.mx_code_bytes(128, 64, 8), dtype=torch.uint8, device=DEV)
+    scales = torch.zeros(lib.mx_scale_bytes(128, 64), dtype=torch.uint8, device=DEV)
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        lib.mx_check(other.cuda_stream)
+        with pytest.raises(lib.QaggError) as e:
+            lib.mx_check(stream())
+        assert "error -4" in str(e.value)
+        lib.mx_quantize(x.data_ptr(), lib.F32, 128, codes.data_ptr(), scales.data_ptr(), 128, 64, lib.MXINT8, False, stream())
+    graph.replay()
+    torch.cuda.synchronize()
+    want = mx_util.pack(x.double().cpu().numpy(), mx_util.INT8)
+    assert np.array_equal(codes.cpu().numpy(), want[0]) and np.array_equal(scales.cpu().numpy(), want[1])

@@ -141,3 +141,10 @@ def test_roles_of_the_gradient_products(tmp_path):
     assert res.returncode == 0, res.stderr
     run = subprocess.run([exe], capture_output=True, text=True, timeout=60)
     assert run.returncode == 0 and "groups ok" in run.stdout, (run.returncode, run.stdout)
+
+
+def test_wait_selftest_refuses_long_limits(lib):
+    for limit in (0, -1, 10 ** 9 + 1):
+        with pytest.raises(lib.QaggError) as e:
+            lib.mx_wait_selftest(limit)
+        assert "error -1" in str(e.value)
