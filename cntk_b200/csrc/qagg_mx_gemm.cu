@@ -637,10 +637,7 @@ __global__ void __launch_bounds__(TT, 1) k_mx_times(const __grid_constant__ CUte
 // integer of at most 12, looked up four at a time by PRMT, so a block's products are integer dot products, exact: with mag the
 // magnitudes of w and x signed, sum w x = sum mag x - 2 * (sum over negative w of mag x).  x is decoded once per CTA, into shared
 // memory.  Only the sum over blocks is in fp32.
-// Chosen up to FEW_PRODUCTS multiply-adds: beyond them its instructions last longer than what the tiles need besides the weights.
-// us, this / tiles:  2048 x 2048, 1 token 2.6 / 4.9, 4 tokens 4.2 / 5.3;  9304 x 4096, 1 token 7.3 / 7.5, 4 tokens 14.8 / 7.5.
-constexpr int FEW = 4, FEW_VALUES = 32768; // tokens; values of x, a byte each in shared memory
-constexpr long long FEW_PRODUCTS = 36LL << 20;
+// When it is chosen: times_few.
 
 // four codes (16 bits) -> magnitudes times two; mask: 0xff where the code is negative, 0x80 where not
 __device__ __forceinline__ unsigned fp4_magnitudes(unsigned c, unsigned& mask)
@@ -1573,7 +1570,7 @@ int qagg_mx_times(void* stream, const void* w_codes, const void* w_scales, const
     rc = launch_cfg_for_current_device(&cfg);
     if (rc)
         return rc;
-    if (T <= FEW && K > 0 && (T == 3 ? 4 : T) * K <= FEW_VALUES && T * O * K <= FEW_PRODUCTS)
+    if (times_few(O, T, K))
     {
         const auto few = [&](auto* p) { return launch_times_few((cudaStream_t) stream, w_codes, w_scales, x_codes, x_scales, bias, p, ld_y, O, (int) T, K, cfg.numSMs); };
         return check_cuda(y_type == QAGG_F32 ? few((float*) y) : y_type == QAGG_F16 ? few((__half*) y) : few((__nv_bfloat16*) y), "4-bit product kernel launch");

@@ -1,5 +1,5 @@
-// qagg_mx_groups.h -- how the gradient products (qagg_mx_gemm.cu) divide a CTA's warps, registers and tensor memory.  Plain constants, so that a
-// host compiler can check them.
+// qagg_mx_groups.h -- how the gradient products (qagg_mx_gemm.cu) divide a CTA's warps, registers and tensor memory, and which kernel a 4-bit
+// product takes.  Nothing here needs a device compiler, so that a host compiler can check it.
 #pragma once
 
 namespace qagg {
@@ -36,5 +36,18 @@ struct GradGroups
     static constexpr int convArrivals = PAIR ? 8 : 4, denseArrivals = DENSE ? 4 * load * (PAIR ? 2 : 1) : 1, takenArrivals = 4 * result * (PAIR ? 2 : 1);
     static_assert(convArrivals >= 1 && denseArrivals >= 1 && takenArrivals >= 1, "barrier counts");
 };
+
+// A 4-bit product y (O x T) of K inputs: by the kernel for a few tokens, or by tiles on the tensor cores?  The few tokens' x, a byte a value,
+// stays in shared memory.  Two tokens at most: until the integer dot products last longer than what the tiles need besides the weights.
+// Three and four (both computed as four) bring twice the work for the same weights, and cross the tiles earlier.
+// us, this / tiles, weights in L2:  1 token 2048 x 2048 2.4 / 4.8, 9304 x 2048 4.5 / 6.2, 9304 x 4096 6.8 / 7.1, 9304 x 4608 8.0 / 7.7;
+// 2 tokens 9304 x 2048 5.5 / 6.3, 4096 x 4096 6.0 / 5.9, 12288 x 2048 7.4 / 6.3;  4 tokens 2048 x 2048 4.0 / 5.0, 9304 x 512 5.7 / 4.1,
+// 2048 x 4096 5.9 / 5.8, 4096 x 2048 5.7 / 5.1.  With the weights in HBM both take half a microsecond to a whole one more.
+constexpr long long FEW = 4, FEW_VALUES = 32768;
+constexpr bool times_few(long long O, long long T, long long K)
+{
+    const long long t = T == 3 ? 4 : T;
+    return T >= 1 && T <= FEW && K > 0 && t * K <= FEW_VALUES && t * O * K <= (T <= 2 ? 38LL << 20 : 16LL << 20);
+}
 
 } // namespace qagg

@@ -1,4 +1,5 @@
-// mx_groups_check.cpp -- the constants by which the gradient products divide a CTA.  Exit code 0 = all hold.
+// mx_groups_check.cpp -- the constants by which the gradient products divide a CTA, and the choice of the 4-bit product's kernel.  Exit code
+// 0 = all hold.
 #include <cstdio>
 
 #include "../../cntk_b200/csrc/qagg_mx_groups.h"
@@ -31,6 +32,21 @@ int main()
     for (int i = 0; i < 4; ++i)
         if (rc[i])
             return 10 * (i + 1) + rc[i];
+    // where one kernel was measured to be clearly ahead, it is the one that is taken
+    const struct
+    {
+        long long O, T, K;
+        bool few;
+    } measured[] = {{2048, 1, 2048, true}, {9304, 1, 2048, true}, {9304, 1, 4096, true}, {12288, 1, 4096, false}, {16384, 1, 4096, false}, {2048, 2, 2048, true},
+                    {9304, 2, 2048, true}, {12288, 2, 2048, false}, {9304, 2, 4096, false}, {2048, 3, 2048, true}, {2048, 4, 2048, true}, {9304, 3, 512, false},
+                    {9304, 4, 512, false}, {4096, 3, 2048, false}, {4096, 4, 2048, false}, {9304, 4, 1024, false}, {33, 4, 8192, true}};
+    for (const auto& m : measured)
+        if (qagg::times_few(m.O, m.T, m.K) != m.few)
+            return 100;
+    // x has to fit; nothing to multiply, or more tokens, is the tiles' business
+    if (qagg::times_few(33, 4, 8193) || qagg::times_few(33, 3, 8193) || qagg::times_few(20, 1, 32769) || !qagg::times_few(20, 1, 32768) || qagg::times_few(20, 1, 0) ||
+        qagg::times_few(20, 5, 32) || qagg::times_few(1LL << 29, 1, 32768))
+        return 101;
     std::puts("groups ok");
     return 0;
 }
