@@ -968,3 +968,122 @@ def test_check_beside_a_capture(lib):
     torch.cuda.synchronize()
     want = mx_util.pack(x.double().cpu().numpy(), mx_util.INT8)
     assert np.array_equal(codes.cpu().numpy(), want[0]) and np.array_equal(scales.cpu().numpy(), want[1])
+
+
+@pytest.mark.parametrize("t,O,I,T,chain", [("bf16", 128, 128, 32768, 32), ("bf16", 2304, 2304, 8192, 32), ("bf16", 1280, 2304, 16384, 64), ("bf16", 2303, 4096, 8192, 32),
+                                           ("f32", 2304, 4096, 4096, 32), ("f32", 130, 128, 8192, 32), ("f16", 2304, 4096, 4096, 32)])
+def test_long_sums_of_the_weight_gradient(lib, t, O, I, T, chain):
+    """16 products an instruction, split and whole, by single CTAs and by pairs (64 instructions where dy is bf16), with and without loaders."""
+    small = 0.75 * UNIT / 16
+    up = 2.0 ** 14 if t == "f16" else 1.0  # fp16 holds no 2^-28: all values larger
+    dy = torch.full((T, O), small * up, dtype=TYPES[t], device=DEV)
+    dy[0] = up
+    xc, xs = ones(lib, I, T, lib.MXINT8)
+    dw = torch.zeros(I, O, device=DEV)
+    lib.mx_weight_grad(dy.data_ptr(), code(lib, t), O, xc.data_ptr(), xs.data_ptr(), lib.MXINT8, dw.data_ptr(), O, I, T, False, stream())
+    lib.mx_check(stream())
+    least, most = lost(dw / up, 1.0 + (T - 1) * small)
+    # the first instruction has 15 small values: a sixteenth of 3/4 unit that the total lacks
+    assert least >= -0.5 and most <= 0.75 * chain + 0.5
+
+
+@pytest.mark.parametrize("t,O,I,T,chain", [("bf16", 32768, 128, 64, 32), ("bf16", 8192, 1280, 2304, 32), ("bf16", 8192, 2048, 2048, 64), ("f32", 4096, 2304, 4096, 32),
+                                           ("f16", 4096, 2304, 4096, 32)])
+def test_long_sums_of_the_input_gradient(lib, t, O, I, T, chain):
+    small = 0.75 * UNIT / 16
+    up = 2.0 ** 14 if t == "f16" else 1.0
+    dy = torch.full((T, O), small * up, dtype=TYPES[t], device=DEV)
+    dy[:, 0] = up
+    wc, ws = ones(lib, I, O, lib.MXFP4)
+    dx = torch.zeros(T, I, device=DEV)
+    lib.mx_input_grad(dy.data_ptr(), code(lib, t), O, wc.data_ptr(), ws.data_ptr(), lib.MXFP4, dx.data_ptr(), lib.F32, I, O, I, T, stream())
+    lib.mx_check(stream())
+    least, most = lost(dx / up, 1.0 + (O - 1) * small)
+    assert least >= -0.5 and most <= 0.75 * chain + 0.5
+
+
+@pytest.mark.parametrize("weight", [True, False])
+@pytest.mark.parametrize("t,D", [("f32", (2304, 4096, 4096)), ("f32", (200, 130, 2048)), ("f16", (2304, 4096, 4096)), ("f16", (200, 130, 2048))])
+def test_every_plane_of_dy_counts(lib, t, D, weight):
+    """Values of one sign with all significant bits set.  fp32: the last of three bf16 terms is 2^-16 of the value, fp16: the second of two is
+    7 * 2^-11; the sum's own error is below both: chains of 24 (fp16: 32) instructions, each off by a unit of the sum so far, half the
+    chain's sum on average (16.5 units), and at most 96 chains, each addition off by half a unit of the sum so far (24 units)."""
+    v = 2.0 - 2.0 ** -23 if t == "f32" else 2.0 - 2.0 ** -10
+    A, B, C = D  # results A x B, contraction C
+    dy = torch.full((C, A) if weight else (B, C), v, dtype=TYPES[t], device=DEV)
+    out = torch.zeros((B, A), device=DEV)
+    if weight:
+        xc, xs = ones(lib, B, C, lib.MXINT8)
+        lib.mx_weight_grad(dy.data_ptr(), code(lib, t), A, xc.data_ptr(), xs.data_ptr(), lib.MXINT8, out.data_ptr(), A, B, C, False, stream())
+    else:
+        wc, ws = ones(lib, A, C, lib.MXFP4)
+        lib.mx_input_grad(dy.data_ptr(), code(lib, t), C, wc.data_ptr(), ws.data_ptr(), lib.MXFP4, out.data_ptr(), lib.F32, A, C, A, B, stream())
+    lib.mx_check(stream())
+    want = v * C
+    worst = max(abs(float(out.max()) - want), abs(float(out.min()) - want))
+    assert worst <= 41 * UNIT * want  # 4.9e-6; without the last plane 1.5e-5 (fp16: 1.7e-3)
+    assert worst < 2.0 ** -17 * want
+
+
+@pytest.mark.parametrize("O,I,T,t", [(2304, 4096, 8192, "f32"), (1280, 2304, 16384, "bf16"), (128, 128, 32768, "bf16"), (130, 140, 32768, "f16")])
+def test_sums_of_one_sign(lib, O, I, T, t):
+    """Random values of one sign: what a chain of n (64 at most) truncating instructions loses, a unit of the sum so far each, is on average
+    half of n units of the chain's sum; the additions of m chains, half a unit of the sum so far, a quarter of m units at most."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    dy = (torch.rand(T, O, device=DEV, generator=g) + 0.5).to(TYPES[t])
+    x = torch.rand(T, I, device=DEV, generator=g) + 0.5
+    xc, xs = quantized(lib, x, I, T, I, "f32", lib.MXINT8)
+    values = torch.zeros(T, I, device=DEV)
+    lib.mx_unquantize(xc.data_ptr(), xs.data_ptr(), values.data_ptr(), lib.F32, I, I, T, lib.MXINT8, stream())
+    dw = torch.zeros(I, O, device=DEV)
+    lib.mx_weight_grad(dy.data_ptr(), code(lib, t), O, xc.data_ptr(), xs.data_ptr(), lib.MXINT8, dw.data_ptr(), O, I, T, False, stream())
+    rows = torch.arange(0, I, max(1, I // 64), device=DEV)
+    want = values[:, rows].double().t() @ dy.double()
+    planes = {"bf16": 1, "f16": 2, "f32": 3}[t]
+    pair = t == "bf16" and O == 1280
+    n = 64 if pair else 32 // (4 * planes) * 4 * planes
+    m = T * planes / 16 / n
+    assert float((dw[rows].double() / want - 1).abs().max()) <= (n / 2 + 2 + m / 4) * UNIT
+
+
+@pytest.mark.parametrize("t,t2", [("f32", "f16"), ("f32", "bf16"), ("f16", "bf16"), ("bf16", "f16")])
+@pytest.mark.parametrize("fmt", [mx_util.FP4, mx_util.INT8])
+@pytest.mark.parametrize("O,I,T,pad,offset", [(132, 512, 256, 0, 0), (257, 129, 300, 7, 1), (520, 2304, 4096, 0, 0)])
+def test_input_grad_of_another_type(lib, O, I, T, pad, offset, fmt, t, t2):
+    """dx of a 16-bit type that is not dy's."""
+    rng = np.random.default_rng(O + I + T)
+    _, d, dy = dense(rng, T, O, t, pad, offset, 1e-2)
+    (wc, ws), w = packed(rng, O, I, fmt, 0.05)
+    flat, dx = room(T, I, t2, pad, offset)
+    lib.mx_input_grad(d.data_ptr(), code(lib, t), O + pad, wc.data_ptr(), ws.data_ptr(), fmt, dx.data_ptr(), code(lib, t2), I + pad, O, I, T, stream())
+    lib.mx_check(stream())
+    check(dx, dy @ w, np.abs(dy) @ np.abs(w), {"bf16": 1, "f16": 2, "f32": 3}[t] * O / 16, t2, "input gradient")
+    untouched(flat, dx, pad, offset)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("O,T,K", [(130, 40, 40000), (200, 130, 20000), (4096, 2304, 8448)])
+def test_times_with_several_chains(lib, O, T, K, t):
+    """Contractions that hand the accumulator over within a tile, at every width: 64, 128 and 256."""
+    rng = np.random.default_rng(K)
+    (wc, ws), w = packed(rng, O, K, mx_util.FP4, 0.05)
+    (xc, xs), x = packed(rng, T, K, mx_util.FP4)
+    y = torch.zeros(T, O, dtype=TYPES[t], device=DEV)
+    lib.mx_times(wc.data_ptr(), ws.data_ptr(), xc.data_ptr(), xs.data_ptr(), 0, y.data_ptr(), code(lib, t), O, O, T, K, stream())
+    lib.mx_check(stream())
+    check(y, x @ w.T, np.abs(x) @ np.abs(w).T, K / 16, t, "times")
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("O,T,K,pad", [(9304, 1, 1100, 0), (7105, 1, 64, 3), (9304, 2, 2048, 0), (7200, 2, 429, 5), (7111, 4, 96, 0)])
+def test_times_of_few_tokens_and_many_outputs(lib, O, T, K, pad, t):
+    """Two rows a warp, 32 apart: the last ones beyond the matrix too."""
+    rng = np.random.default_rng(O + K)
+    (wc, ws), w = packed(rng, O, K, mx_util.FP4, 0.05)
+    (xc, xs), x = packed(rng, T, K, mx_util.FP4)
+    bias = rng.standard_normal(O).astype(np.float32)
+    bd = torch.from_numpy(bias).to(DEV)
+    flat, y = room(T, O, t, pad)
+    lib.mx_times(wc.data_ptr(), ws.data_ptr(), xc.data_ptr(), xs.data_ptr(), bd.data_ptr(), y.data_ptr(), code(lib, t), O + pad, O, T, K, stream())
+    check(y, x @ w.T + bias, np.abs(x) @ np.abs(w).T + np.abs(bias), K / 16, t, "times")
+    untouched(flat, y, pad, 0)
