@@ -901,6 +901,8 @@ static int check_act(const char* who, const void* a, int64_t lda, const void* b,
         return QAGG_OK;
     if (!a || !b || !codes || !scales)
         return fail(QAGG_EINVAL, std::string(who) + ": null pointer");
+    if (a == b && lda != ldb && N > 1)
+        return fail(QAGG_EINVAL, std::string(who) + ": in place the two ld must be the same");
     if ((((uintptr_t) codes | (uintptr_t) scales) & 15) || (((uintptr_t) a | (uintptr_t) b) & (mx_type_bytes(type) - 1)))
         return fail(QAGG_EINVAL, std::string(who) + ": codes and scales must be 16-byte aligned, the others aligned to their type");
     return QAGG_OK;

@@ -148,3 +148,12 @@ def test_wait_selftest_refuses_long_limits(lib):
         with pytest.raises(lib.QaggError) as e:
             lib.mx_wait_selftest(limit)
         assert "error -1" in str(e.value)
+
+
+def test_in_place_layers_need_one_ld(lib):
+    """y over x and dx over dy with another distance between columns would overwrite columns that are still to be read."""
+    p = 4096
+    for call in (lambda: lib.mx_act_forward(p, lib.F32, 64, lib.ACT_RELU, p, 72, p, p, 64, 8), lambda: lib.mx_act_backward(p, lib.F32, 72, p, p, lib.ACT_RELU, p, 64, 64, 8)):
+        with pytest.raises(lib.QaggError) as e:
+            call()
+        assert "error -1" in str(e.value) and "in place" in str(e.value)
