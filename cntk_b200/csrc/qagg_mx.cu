@@ -822,15 +822,19 @@ extern "C" {
 
 int64_t qagg_mx_code_bytes(int64_t M, int64_t N, int format)
 {
-    if (M < 0 || N < 0 || !format_ok(format))
-        return fail(QAGG_EINVAL, "qagg_mx_code_bytes: bad arguments");
+    const int rc = mx_check_dims("qagg_mx_code_bytes", M, N);
+    if (rc)
+        return rc;
+    if (!format_ok(format))
+        return fail(QAGG_EINVAL, "qagg_mx_code_bytes: unknown format");
     return N * mx_pitch(M, format);
 }
 
 int64_t qagg_mx_scale_bytes(int64_t M, int64_t N)
 {
-    if (M < 0 || N < 0)
-        return fail(QAGG_EINVAL, "qagg_mx_scale_bytes: bad arguments");
+    const int rc = mx_check_dims("qagg_mx_scale_bytes", M, N);
+    if (rc)
+        return rc;
     return (N + 127) / 128 * mx_scale_tiles(M) * 512;
 }
 

@@ -157,3 +157,13 @@ def test_in_place_layers_need_one_ld(lib):
         with pytest.raises(lib.QaggError) as e:
             call()
         assert "error -1" in str(e.value) and "in place" in str(e.value)
+
+
+def test_sizes_beyond_the_limits_are_refused(lib):
+    """A matrix that no call takes has no size: the products would not fit 64 bits."""
+    for m, n in ((1 << 62, 8), ((1 << 63) - 1, 1), (1 << 40, 1 << 40), (1 << 30, 1), (1, 65535 * 128 + 1), (1, 1 << 62)):
+        for call in (lambda: lib.mx_code_bytes(m, n, lib.MXINT8), lambda: lib.mx_scale_bytes(m, n)):
+            with pytest.raises(lib.QaggError) as e:
+                call()
+            assert "error -1" in str(e.value)
+    assert lib.mx_code_bytes((1 << 30) - 1, 65535 * 128, lib.MXINT8) == (1 << 30) * 65535 * 128
