@@ -1,5 +1,5 @@
-// qagg_mx.cuh -- the microscaled (MX) matrix form shared by qagg_mx.cu (quantize, unquantize, activations), qagg_mx_times.cu
-// (4-bit product) and qagg_mx_grad.cu (gradients from packed operands).
+// qagg_mx.cuh -- the microscaled (MX) matrix form shared by qagg_mx.cu (quantize, unquantize, activations) and qagg_mx_gemm.cu (4-bit
+// product, gradients from packed operands).
 //
 // A packed M x N matrix has blocks of 32 rows in each column.  A block shares the scale 2^X, kept as the byte X + 127 (255: the
 // block held a NaN or an infinity, every value of it is NaN), and value = element * 2^X with

@@ -9,8 +9,8 @@
 // Both: 128 x n output tiles, dealt to one resident CTA per SM.  A copy warp feeds a ring of shared-memory stages and runs ahead into
 // the next tile, one thread issues the products, eight (or four) result warps hold the tile's sums in registers.
 //
-// The sums.  The tensor cores add to their fp32 accumulator with truncation: sums of n instructions come out low by up to n / 2 units in
-// the last place, 6.8e-6 of the result after 512 of them.  So where the output is fp32 a chain ends after CHAIN instructions; the
+// The sums.  The tensor cores add to their fp32 accumulator with truncation: n instructions lose less than n units of 2^-23 of the
+// largest sum on the way, 6.8e-6 of a sum of positive values after 512 of them.  So a chain ends after CHAIN instructions where the output is fp32; the
 // result warps add its value to their registers (round to nearest) and hand the accumulator back, which takes about 2000 cycles
 // from the last product to the next.  Two accumulators in turn hide that, and the next tile begins while this one is being
 // written.  (A 256-wide tile of the 4-bit product has room for one.)
@@ -58,8 +58,8 @@ constexpr int GEMM_SMEM_MAX = 224 * 1024; // dynamic; barriers and scales take a
 // barriers.
 constexpr int GEMM_SMEM_MIN = 200 * 1024;
 // Tensor-core instructions in a row on one accumulator.  After 32 the sums are within 3e-7; with a single accumulator, where every
-// chain costs its hand-over, 64 are taken: within 6e-7, as a sum in plain fp32 is.  n instructions lose less than n units of 2^-23.  A
-// 16-bit result's own rounding is half a step: 4096 such units for fp16, 32768 for bf16; chains for them lose a 32nd of that at most.
+// chain costs its hand-over, 64 are taken: within 6e-7, as a sum in plain fp32 is.  A 16-bit result's own rounding is half a step: 4096
+// units of 2^-23 for fp16, 32768 for bf16; chains for them lose a 32nd of that at most.
 constexpr int CHAIN = 32, CHAIN_SINGLE = 64, CHAIN_FP16 = 128, CHAIN_BF16 = 1024;
 template <class T, bool SINGLE>
 constexpr int CHAIN_OF = std::is_same_v<T, __half> ? CHAIN_FP16 : std::is_same_v<T, __nv_bfloat16> ? CHAIN_BF16 : SINGLE ? CHAIN_SINGLE : CHAIN;

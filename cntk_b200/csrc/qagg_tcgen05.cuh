@@ -1,5 +1,5 @@
-// qagg_tcgen05.cuh -- device helpers of the kernels that multiply on the fifth-generation tensor cores (qagg_mx_times.cu,
-// qagg_mx_grad.cu): tensor memory, shared-memory operand descriptors, instruction descriptors, bounded waits.
+// qagg_tcgen05.cuh -- device helpers of the kernels that multiply on the fifth-generation tensor cores (qagg_mx_gemm.cu): tensor
+// memory, shared-memory operand descriptors, instruction descriptors, bounded waits.
 #pragma once
 
 #include "qagg_async.cuh"
@@ -9,9 +9,9 @@
 namespace qagg {
 
 // ---- waits ------------------------------------------------------------------------------------------------------------------
-// try_wait suspends the thread for a while in hardware before it answers.  A wait that has lasted TC_WAIT_NS (the end of the longest
-// product a call can ask for is a tenth of a second away) gives up: *broken ends every later wait of the CTA at once, the status
-// word tells the host.
+// try_wait suspends the thread for a while in hardware before it answers.  A wait is for one stage of a ring or one chain of products, a
+// few microseconds however long the product as a whole; one that has lasted TC_WAIT_NS gives up: *broken ends every later wait of the
+// CTA at once, the status word tells the host.
 constexpr unsigned long long TC_WAIT_NS = 4000000000ull;
 __device__ __forceinline__ unsigned long long clock_ns()
 {
