@@ -60,6 +60,8 @@ constexpr int GEMM_SMEM_MIN = 200 * 1024;
 // Tensor-core instructions in a row on one accumulator.  After 32 the sums are within 3e-7; with a single accumulator, where every
 // chain costs its hand-over, 64 are taken: within 6e-7, as a sum in plain fp32 is.  A 16-bit result's own rounding is half a step: 4096
 // units of 2^-23 for fp16, 32768 for bf16; chains for them lose a 32nd of that at most.
+// The planes of an fp32 or fp16 dy count as instructions of their own.  A step takes the smallest plane first: the other way round all
+// twelve instructions of an fp32 step truncated a sum that the first four had made large (132 x 512 x 256: 3.9e-7, so 7e-8).
 constexpr int CHAIN = 32, CHAIN_SINGLE = 64, CHAIN_FP16 = 128, CHAIN_BF16 = 1024;
 template <class T, bool SINGLE>
 constexpr int CHAIN_OF = std::is_same_v<T, __half> ? CHAIN_FP16 : std::is_same_v<T, __nv_bfloat16> ? CHAIN_BF16 : SINGLE ? CHAIN_SINGLE : CHAIN;
@@ -1093,13 +1095,13 @@ __global__ void __launch_bounds__(GradGroups<(DENSE > 0), PAIR>::threads, 1) k_m
                     const unsigned ta = tmA + slot * 32, acc = tm + chain.buf * WIDEST;
                     slot = (slot + 1) % SLOTS;
 #pragma unroll
-                    for (int p = 0; p < NP; ++p)
+                    for (int p = NP - 1; p >= 0; --p) // small planes first, onto small sums: see CHAIN
 #pragma unroll
                         for (int j = 0; j < GK / 16; ++j)
                             if constexpr (PAIR)
-                                mma_bf16_ts_pair(acc, ta + j * 8, d + p * (share * 128 >> 4) + j * KSTEP, idesc, inChain > 0 || p + j > 0);
+                                mma_bf16_ts_pair(acc, ta + j * 8, d + p * (share * 128 >> 4) + j * KSTEP, idesc, inChain > 0 || p < NP - 1 || j > 0);
                             else
-                                mma_bf16_ts(acc, ta + j * 8, d + p * (share * 128 >> 4) + j * KSTEP, idesc, inChain > 0 || p + j > 0);
+                                mma_bf16_ts(acc, ta + j * 8, d + p * (share * 128 >> 4) + j * KSTEP, idesc, inChain > 0 || p < NP - 1 || j > 0);
                     if constexpr (PAIR)
                         tc_commit_pair(&bars.empty[ring.s]);
                     else

@@ -400,7 +400,7 @@ int qagg_mx_times(void* stream, const void* w_codes, const void* w_scales, const
  * dy is O x T.  The packed values are exact in the product; fp16 and fp32 dy are taken as exact sums of two and three bf16 terms
  * (magnitudes below about 2^-109 lose their last bits).
  * Precision of both and of qagg_mx_times: the tensor cores truncate their running sum after every 16 (times: 64) values.  For an fp32
- * result at most 64 such steps follow one another before they are added in fp32 to nearest: 3e-7 to 6e-7 of a long sum of
+ * result at most 64 such steps follow one another before they are added in fp32 to nearest: 1e-7 to 8e-7 of a long sum of
  * positive values, 64 units of 2^-23 of the largest partial sum at the very worst.  For fp16 results they are 128, for bf16 1024, which is
  * a 32nd of half a step of the type at worst. */
 int qagg_mx_weight_grad(void* stream, const void* dy, int dy_type, int64_t ld_dy, const void* x_codes, const void* x_scales, int format, float* dw, int64_t O, int64_t I,

@@ -1087,3 +1087,21 @@ def test_times_of_few_tokens_and_many_outputs(lib, O, T, K, pad, t):
     lib.mx_times(wc.data_ptr(), ws.data_ptr(), xc.data_ptr(), xs.data_ptr(), bd.data_ptr(), y.data_ptr(), code(lib, t), O + pad, O, T, K, stream())
     check(y, x @ w.T + bias, np.abs(x) @ np.abs(w).T + np.abs(bias), K / 16, t, "times")
     untouched(flat, y, pad, 0)
+
+
+@pytest.mark.parametrize("weight", [True, False])
+@pytest.mark.parametrize("A,B", [(130, 40), (2304, 4096)])
+def test_small_planes_are_added_first(lib, A, B, weight):
+    """64 values 1 + 3 * 2^-23, in bf16 terms 1 and 3 * 2^-23.  The small ones first: 3 * 2^-17, then four times 16, all of it exact in 24 bits.
+    The large ones first make 64, whose unit is 2^-17: each of four instructions with 3/4 of it is lost."""
+    C = 64
+    dy = torch.full((C, A) if weight else (B, C), 1.0 + 3 * UNIT, device=DEV)
+    out = torch.zeros((B, A), device=DEV)
+    if weight:
+        xc, xs = ones(lib, B, C, lib.MXINT8)
+        lib.mx_weight_grad(dy.data_ptr(), lib.F32, A, xc.data_ptr(), xs.data_ptr(), lib.MXINT8, out.data_ptr(), A, B, C, False, stream())
+    else:
+        wc, ws = ones(lib, A, C, lib.MXFP4)
+        lib.mx_input_grad(dy.data_ptr(), lib.F32, C, wc.data_ptr(), ws.data_ptr(), lib.MXFP4, out.data_ptr(), lib.F32, A, C, A, B, stream())
+    lib.mx_check(stream())
+    assert bool((out == 64.0 + 3 * 2.0 ** -17).all())
