@@ -1105,3 +1105,32 @@ def test_small_planes_are_added_first(lib, A, B, weight):
         lib.mx_input_grad(dy.data_ptr(), lib.F32, C, wc.data_ptr(), ws.data_ptr(), lib.MXFP4, out.data_ptr(), lib.F32, A, C, A, B, stream())
     lib.mx_check(stream())
     assert bool((out == 64.0 + 3 * 2.0 ** -17).all())
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16", "f32"])
+def test_fp16_results_with_several_chains(lib, t):
+    """Chains for fp16 results end within these contractions: pairs with one accumulator (bf16 dy, the product) and loaders with two."""
+    O, I, T = 4200, 2048, 2100
+    rng = np.random.default_rng(17)
+    _, d, dy = dense(rng, T, O, t, 0, 0, 1e-2)
+    (wc, ws), w = packed(rng, O, I, mx_util.FP4, 0.05)
+    dx = torch.zeros(T, I, dtype=torch.float16, device=DEV)
+    lib.mx_input_grad(d.data_ptr(), code(lib, t), O, wc.data_ptr(), ws.data_ptr(), 4, dx.data_ptr(), lib.F16, I, O, I, T, stream())
+    lib.mx_check(stream())
+    check(dx, dy @ w, np.abs(dy) @ np.abs(w), {"bf16": 1, "f16": 2, "f32": 3}[t] * O / 16, "f16", "input gradient")
+
+
+def test_product_for_fp16_with_several_chains(lib):
+    O, T, K = 2304, 4096, 16640
+    g = torch.Generator(device=DEV).manual_seed(5)
+    w, x = torch.randn(K, O, device=DEV, generator=g) * 0.05, torch.randn(T, K, device=DEV, generator=g)
+    wq, xq = quantized(lib, w, O, K, O, "f32", lib.MXFP4, True), quantized(lib, x, K, T, K, "f32", lib.MXFP4)
+    wv, xv = torch.zeros(O, K, device=DEV), torch.zeros(T, K, device=DEV)
+    lib.mx_unquantize(wq[0].data_ptr(), wq[1].data_ptr(), wv.data_ptr(), lib.F32, K, K, O, lib.MXFP4, stream())
+    lib.mx_unquantize(xq[0].data_ptr(), xq[1].data_ptr(), xv.data_ptr(), lib.F32, K, K, T, lib.MXFP4, stream())
+    y = torch.zeros(T, O, dtype=torch.float16, device=DEV)
+    lib.mx_times(wq[0].data_ptr(), wq[1].data_ptr(), xq[0].data_ptr(), xq[1].data_ptr(), 0, y.data_ptr(), lib.F16, O, O, T, K, stream())
+    lib.mx_check(stream())
+    rows = torch.arange(0, T, 37, device=DEV)
+    want, mags = xv[rows].double() @ wv.double().t(), xv[rows].abs().double() @ wv.abs().double().t()
+    check(y[rows], want.cpu().numpy(), mags.cpu().numpy(), K / 16, "f16", "times")
